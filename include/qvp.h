@@ -313,6 +313,214 @@ QVP_API int qvp_kv_append(void* pool, size_t block_stride, uint32_t num_blocks,
                   int32_t* error_word, qvp_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Sparse attention over the paged cache.
+ *
+ * A decode step that reads only the blocks worth reading, in three calls:
+ *
+ *   qvp_rope_append      rotates the new tokens' queries and keys, writes keys
+ *                        and values into the pool and brings the summaries of
+ *                        the blocks they land in up to date
+ *   qvp_select_blocks    scores every block of a context by its summary and
+ *                        lists the best ones of each (sequence, kv head)
+ *   qvp_decode_selected  qvp_decode over the listed blocks alone
+ *
+ * and qvp_summarize_blocks, which makes the summaries of a cache that
+ * qvp_kv_append, a swap-in or a host copy filled.
+ *
+ * Summary of a block, for one layer and kv head: the minimum and the maximum
+ * over its filled token slots of every channel of K, in the pool's element
+ * type, each channel by itself. Summaries live in a pool of their own with
+ * one block per block of the cache, under the same id: the pool of
+ * qvp_summary_shape(shape), whose elements are ordered
+ * [layer][kv_head][min|max][head_dim]. qvp_pool_create makes it, and
+ * qvp_copy_blocks, qvp_gather_blocks and qvp_scatter_blocks move it, with the
+ * ids of the cache: a caller that copies or swaps blocks of the cache does the
+ * same to their summaries, or makes them again.
+ *
+ * None of the calls needs a workspace or keeps state, so calls on different
+ * streams, and graphs that captured them, are independent as long as their
+ * buffers are. All take the current device's pointers. dtype is the type of
+ * the pool, the summaries, q, k, v and the outputs; head_dim <= 256.
+ * Lengths, tables and lists are read on the device only: entries that are
+ * wrong set bits of *error_word (1: an id outside the pool or a list entry
+ * past the context; 4: a length out of range) and are skipped, so no access
+ * leaves the pool. The block id -1 past a context is never read. No
+ * counterpart in the reference (it attends every token).
+ * ------------------------------------------------------------------------- */
+
+/* The block shape of the summary pool of a cache with blocks of `shape`. */
+QVP_API int qvp_summary_shape(const qvp_block_shape* shape, qvp_block_shape* summary);
+
+/*
+ * qvp_rope_append: for every sequence b, its query_lens[b] newest tokens take
+ * the cache positions context_lens[b] - query_lens[b] + t (t = 0, 1, ...), the
+ * rows and lengths of qvp_prefill. For token t:
+ *   query_out[b][t][h] = R(query[b][t][h])            for every query head
+ *   K slot             = R(key[b][t][g])              for every kv head
+ *   V slot             = value[b][t][g]
+ * R turns the pairs (x_p, y_p), p < rotary_dim / 2, of a head's first
+ * rotary_dim elements by the angle a_p = pos * inv_freq[p]:
+ *   (x, y) -> (x cos a - y sin a, y cos a + x sin a)
+ * and leaves the others. A pair is elements (p, p + rotary_dim/2), or (2p,
+ * 2p + 1) with rotary_interleaved. pos is rope_positions[axis][b][t], where
+ * the first rope_sections[0] pairs take axis 0, the next rope_sections[1]
+ * axis 1 and so on (the temporal, height and width axes of image and video
+ * tokens; one axis and one section for plain text); with rope_positions NULL
+ * it is the cache position. Angles are formed and reduced in 64 bits, so far
+ * positions keep their accuracy; sums are 32-bit and each result is rounded
+ * to the element type once.
+ *
+ * With `summary`, the summary of each block that holds one of the new tokens
+ * becomes that of its slots up to position context_lens[b] - 1, earlier
+ * tokens of the block included (they are read from the pool, so tokens that
+ * were appended over leave no trace).
+ *
+ * Rows of a token start `*_pitch` elements apart, [batch][max_query_len]
+ * tokens deep (0 = dense rows of heads * head_dim), so q, k and v may be
+ * slices of one projection's output; query_out is dense. query_out may be
+ * query itself when its rows are dense, and overlaps no other buffer. Rows t
+ * >= query_lens[b] are neither read nor written, and query_lens[b] = 0 leaves
+ * a sequence out. num_query_heads = 0 appends keys and values only;
+ * rotary_dim = 0 rotates nothing. The blocks written must belong to one
+ * sequence of the call each (copy-on-write first).
+ */
+#define QVP_ROPE_MAX_AXES 4
+typedef struct qvp_rope_append_args {
+    void* pool;                    /* device base of the block pool            */
+    size_t block_stride;           /* bytes between physical blocks            */
+    uint32_t num_blocks;           /* pool capacity in blocks                  */
+    qvp_block_shape shape;         /* shape shared by every block              */
+    int32_t dtype;                 /* qvp_dtype of the pool, q, k, v           */
+    uint32_t layer;
+    uint32_t num_query_heads;      /* 0: no queries                            */
+    uint32_t batch;
+    uint32_t max_blocks_per_seq;   /* row pitch of block_tables                */
+    uint32_t max_query_len;        /* token pitch of query, key, value         */
+    const int32_t* block_tables;   /* device int32 [batch][max_blocks_per_seq] */
+    const int32_t* context_lens;   /* device int32 [batch], new tokens included */
+    const int32_t* query_lens;     /* device int32 [batch], 0 .. max_query_len */
+    const void* query;             /* device [batch][max_query_len][Hq][D]     */
+    const void* key;               /* device [batch][max_query_len][Hkv][D]    */
+    const void* value;             /* device [batch][max_query_len][Hkv][D]    */
+    void* query_out;               /* device [batch][max_query_len][Hq][D], dense */
+    size_t query_pitch;            /* elements between tokens, 0 = dense       */
+    size_t key_pitch;
+    size_t value_pitch;
+    uint32_t rotary_dim;           /* even, <= head_dim                        */
+    uint32_t rotary_interleaved;   /* 0: halves, 1: neighbours                 */
+    const float* inv_freq;         /* device f32 [rotary_dim / 2]              */
+    const int32_t* rope_positions; /* device int32 [axes][batch][max_query_len] or NULL */
+    uint32_t rope_axes;            /* 1 .. QVP_ROPE_MAX_AXES (with positions)  */
+    uint32_t rope_sections[QVP_ROPE_MAX_AXES]; /* pairs of each axis; they add up to rotary_dim / 2 */
+    void* summary;                 /* device base of the summary pool, or NULL */
+    size_t summary_stride;         /* bytes between its blocks                 */
+    int32_t* error_word;           /* device int32 or NULL; never cleared here */
+} qvp_rope_append_args;
+
+QVP_API int qvp_rope_append(const qvp_rope_append_args* args, qvp_stream_t stream);
+
+/*
+ * qvp_summarize_blocks: the summaries of blocks first_tokens[b] /
+ * tokens_per_block .. (context_lens[b] - 1) / tokens_per_block of every
+ * sequence, from the K in the pool (first_tokens NULL: all blocks).
+ * context_lens[b] = 0, or first_tokens[b] >= context_lens[b], leaves a
+ * sequence out. Sequences may share blocks that are filled to the same slot.
+ */
+typedef struct qvp_summarize_args {
+    const void* pool;
+    size_t block_stride;
+    uint32_t num_blocks;
+    qvp_block_shape shape;
+    int32_t dtype;
+    uint32_t layer;
+    uint32_t batch;
+    uint32_t max_blocks_per_seq;
+    uint32_t max_context_len;      /* host-known upper bound of context_lens   */
+    const int32_t* block_tables;   /* device int32 [batch][max_blocks_per_seq] */
+    const int32_t* context_lens;   /* device int32 [batch], 0 .. max           */
+    const int32_t* first_tokens;   /* device int32 [batch] or NULL             */
+    void* summary;
+    size_t summary_stride;
+    int32_t* error_word;
+} qvp_summarize_args;
+
+QVP_API int qvp_summarize_blocks(const qvp_summarize_args* args, qvp_stream_t stream);
+
+/*
+ * qvp_select_blocks: for every sequence b and kv head g, with the query heads
+ * h of its group,
+ *   up_d   = sum_h max(q[b][h][d], 0)      down_d = sum_h min(q[b][h][d], 0)
+ *   score(block) = sum_d up_d * max_d(block) + down_d * min_d(block)
+ * which no token of the block exceeds in sum_h <q_h, k>. selected[b][g] lists,
+ * in ascending order, the blocks (numbers within the context, as the columns
+ * of block_tables are) of: the first sink_blocks, the last recent_blocks, and
+ * of the others the best by score until there are max_selected; ties go to
+ * the lower block. A context of no more than max_selected blocks lists them
+ * all and reads no summary. The rest of the row is -1, and all of it for
+ * context_lens[b] = 0. Scores are 64-bit sums, so the choice does not depend
+ * on how the work is split. A score that is NaN (summaries or queries that
+ * hold NaN, or infinities against zeros) counts as +infinity. The summaries
+ * of blocks inside sink and recent are not read. Attention with a negative
+ * scale would need the opposite score.
+ */
+typedef struct qvp_select_args {
+    const void* summary;
+    size_t summary_stride;
+    uint32_t num_blocks;
+    qvp_block_shape shape;         /* of the cache's blocks                    */
+    int32_t dtype;
+    uint32_t layer;
+    uint32_t num_query_heads;
+    uint32_t batch;
+    uint32_t max_blocks_per_seq;
+    uint32_t max_context_len;      /* host-known upper bound of context_lens   */
+    const int32_t* block_tables;   /* device int32 [batch][max_blocks_per_seq] */
+    const int32_t* context_lens;   /* device int32 [batch], 0 .. max           */
+    const void* query;             /* device [batch][Hq][D], rotated           */
+    size_t query_pitch;            /* elements between sequences, 0 = dense    */
+    uint32_t max_selected;         /* entries of a list                        */
+    uint32_t sink_blocks;          /* sink + recent <= max_selected            */
+    uint32_t recent_blocks;
+    int32_t* selected;             /* device int32 [batch][Hkv][max_selected]  */
+    int32_t* error_word;
+} qvp_select_args;
+
+QVP_API int qvp_select_blocks(const qvp_select_args* args, qvp_stream_t stream);
+
+/*
+ * qvp_decode_selected: qvp_decode where the softmax of kv head g of sequence b
+ * runs over the tokens below context_lens[b] of the blocks selected[b][g]
+ * names. Entries below 0 are skipped, in any place; a block that is named
+ * twice counts twice; the order only changes the last bits. A list that
+ * leaves no token (every entry < 0, or context_lens[b] = 0) gives zeros.
+ * Entries past the context set error bit 1 and are skipped; a context_lens
+ * entry out of range sets bit 4 and leaves out[b] as it was. Outputs are
+ * the same bits from call to call.
+ */
+typedef struct qvp_decode_selected_args {
+    const void* pool;
+    size_t block_stride;
+    uint32_t num_blocks;
+    qvp_block_shape shape;
+    int32_t dtype;
+    uint32_t layer;
+    uint32_t num_query_heads;
+    float scale;
+    uint32_t batch;
+    uint32_t max_blocks_per_seq;
+    const int32_t* block_tables;   /* device int32 [batch][max_blocks_per_seq] */
+    const int32_t* context_lens;   /* device int32 [batch]                     */
+    const void* query;             /* device [batch][Hq][D]                    */
+    size_t query_pitch;            /* elements between sequences, 0 = dense    */
+    const int32_t* selected;       /* device int32 [batch][Hkv][max_selected]  */
+    uint32_t max_selected;
+    void* out;                     /* device [batch][Hq][D]                    */
+    int32_t* error_word;
+} qvp_decode_selected_args;
+
+QVP_API int qvp_decode_selected(const qvp_decode_selected_args* args, qvp_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * KV-head sharding across the GPUs of one node (one process per GPU).
  *
  * Each GQA group (a kv head and the num_query_heads/num_kv_heads query heads

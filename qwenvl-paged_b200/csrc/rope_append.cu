@@ -1,0 +1,409 @@
+// Rotary append for B200 (sm_100a): the step between the projections and the
+// paged cache. One launch turns the new tokens' queries and keys by their
+// position angles, writes keys and values into the pool and brings the
+// summaries (per-channel minimum and maximum of K) of the blocks they land in
+// up to date.
+//
+//   pair p of a head: angle a = pos * inv_freq[p]
+//   (x, y) -> (x cos a - y sin a, y cos a + x sin a)
+//
+// Every q, k and v element is read once and written once: the call is bound
+// by HBM for prompts and by latency for single tokens. A CTA takes the new
+// tokens of one cache block (so a block's summary belongs to one CTA) and
+// either its K and V or some of its query heads; it makes the cosines and
+// sines of its tokens once, in shared memory, for all its heads.
+#include "sparse_common.cuh"
+
+namespace qvp {
+
+namespace {
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeTokens = 16;       // tokens whose cosines and sines are held at once
+constexpr int kMaxPairs = 128;        // head_dim <= 256
+
+struct RopeParams {
+    uint8_t* pool;
+    size_t block_stride;
+    const int32_t* tables;
+    const int32_t* ctx;
+    const int32_t* qlen;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* q_out;
+    size_t q_pitch, k_pitch, v_pitch;  // elements between tokens
+    const float* inv_freq;
+    const int32_t* pos;
+    uint8_t* summary;
+    size_t summary_stride;
+    int32_t* err;
+    uint32_t num_blocks;
+    uint32_t pitch;
+    uint32_t capacity;       // tokens a table row can name
+    uint32_t T, layer;
+    uint32_t hq, hkv, D;
+    uint32_t batch, max_q;
+    uint32_t units;          // cache blocks a sequence's new tokens can touch
+    uint32_t heads_per_cta;  // query heads of a CTA with blockIdx.y > 0
+    uint32_t rotary;
+    bool interleaved;
+    uint32_t section_end[QVP_ROPE_MAX_AXES];
+};
+
+// cos and sin of pos * f. The angle is taken modulo a turn in 64 bits, where
+// a position of 2^31 still leaves 2^-22 of a turn; what is left is below half
+// a turn, and 32 bits hold it.
+__device__ __forceinline__ float2 turn(int32_t pos, float f) {
+    constexpr double kInvTwoPi = 0.15915494309189533576888376337251;
+    const double turns = static_cast<double>(pos) * static_cast<double>(f) * kInvTwoPi;
+    const float part = static_cast<float>(2.0 * (turns - rint(turns)));
+    float2 cs;
+    sincospif(part, &cs.y, &cs.x);
+    return cs;
+}
+
+// Item i of a head row: two vectors at elements e0 and e1, turned (the pairs
+// [i * VEC, i * VEC + VEC)) or, past the rotary part, copied.
+template <int VEC>
+struct Item {
+    uint32_t e0, e1;
+    bool turned;
+    __device__ __forceinline__ Item(uint32_t i, uint32_t rotary, bool interleaved) {
+        const uint32_t nrot = rotary / (2 * VEC);
+        turned = i < nrot;
+        if (!turned) {
+            e0 = rotary + 2 * VEC * (i - nrot);
+            e1 = e0 + VEC;
+        } else if (interleaved) {
+            e0 = 2 * VEC * i;
+            e1 = e0 + VEC;
+        } else {
+            e0 = VEC * i;
+            e1 = rotary / 2 + VEC * i;
+        }
+    }
+};
+
+// cs: cos and sin of the item's first pair. Products and their sum are 32-bit;
+// the result is rounded to T once.
+template <typename T, int VEC>
+__device__ __forceinline__ void rotate(Vec<T, VEC>& a, Vec<T, VEC>& b, const float2* cs, bool interleaved) {
+    float x[VEC], y[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const float u = to_float<T>(a.v[j]), w = to_float<T>(b.v[j]);
+        x[j] = u;
+        y[j] = w;
+    }
+    if (VEC > 1 && interleaved) {
+        float flat[2 * VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            flat[j] = x[j];
+            flat[VEC + j] = y[j];
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float2 c = cs[j];
+            const float u = flat[2 * j], w = flat[2 * j + 1];
+            flat[2 * j] = u * c.x - w * c.y;
+            flat[2 * j + 1] = w * c.x + u * c.y;
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            a.v[j] = from_float<T>(flat[j]);
+            b.v[j] = from_float<T>(flat[VEC + j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float2 c = cs[j];
+            a.v[j] = from_float<T>(x[j] * c.x - y[j] * c.y);
+            b.v[j] = from_float<T>(y[j] * c.x + x[j] * c.y);
+        }
+    }
+}
+
+// VEC elements at a time where rows and halves fall on 16-byte boundaries,
+// else one by one. grid (batch * units, 1 + groups of query heads).
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeParams p) {
+    __shared__ float2 cs[kRopeTokens * kMaxPairs];
+    // partial ranges of the token groups of K, two vectors each
+    __shared__ Vec<T, VEC> part[kRopeThreads][4];
+
+    wait_for_previous_kernel();
+    allow_next_kernel();
+    const uint32_t b = blockIdx.x / p.units;
+    const int ctx = p.ctx[b];
+    const int n = p.qlen[b];
+    if (n < 0 || static_cast<uint32_t>(n) > p.max_q || ctx < n || static_cast<uint32_t>(ctx) > p.capacity) {
+        if (threadIdx.x == 0) record_error(p.err, kErrBadContext);
+        return;
+    }
+    const uint32_t first = static_cast<uint32_t>(ctx - n);
+    const uint32_t blk = first / p.T + blockIdx.x % p.units;
+    const uint64_t blk_tok = static_cast<uint64_t>(blk) * p.T;
+    if (n == 0 || blk_tok >= static_cast<uint32_t>(ctx)) return;
+    const uint32_t base = static_cast<uint32_t>(blk_tok);                       // position of the block's slot 0
+    const uint32_t lo = max(first, base);                                       // new positions [lo, hi)
+    const uint32_t hi = min(static_cast<uint32_t>(ctx), base + p.T);
+
+    const bool kv = blockIdx.y == 0;
+    uint8_t* frame = nullptr;
+    int32_t id = 0;
+    if (kv) {
+        id = p.tables[static_cast<size_t>(b) * p.pitch + blk];
+        if (static_cast<uint32_t>(id) >= p.num_blocks) {
+            if (threadIdx.x == 0) record_error(p.err, kErrBadBlockId);
+            return;
+        }
+        frame = p.pool + static_cast<size_t>(id) * p.block_stride;
+    }
+    const uint32_t D = p.D;
+    const uint32_t half = p.rotary / 2;
+    const uint32_t row_items = (D + 2 * VEC - 1) / (2 * VEC);
+    const size_t slot_elems = static_cast<size_t>(p.hkv) * D;                   // elements of one token's K or V
+    T* kslots = reinterpret_cast<T*>(frame) + static_cast<size_t>(p.layer) * 2 * p.T * slot_elems;
+    T* vslots = kslots + p.T * slot_elems;
+    const size_t row0 = static_cast<size_t>(b) * p.max_q;
+
+    // K: a thread owns one item of one kv head and every groups-th token
+    const uint32_t k_items = p.hkv * row_items;
+    uint32_t groups = 1;
+    while (groups < kRopeTokens && groups * 2 * k_items <= kRopeThreads) groups *= 2;
+    const uint32_t h0 = kv ? 0u : (blockIdx.y - 1) * p.heads_per_cta;
+    const uint32_t nh = kv ? p.hkv : min(p.heads_per_cta, p.hq - h0);
+
+    for (uint32_t t0 = lo; t0 < hi; t0 += kRopeTokens) {
+        const uint32_t cnt = min(static_cast<uint32_t>(kRopeTokens), hi - t0);
+        const uint32_t row = t0 - first;                                        // token row of t0
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < cnt * half; i += kRopeThreads) {
+            const uint32_t t = i / half, pr = i % half;
+            int32_t pos = static_cast<int32_t>(t0 + t);
+            if (p.pos != nullptr) {
+                uint32_t axis = 0;
+                while (pr >= p.section_end[axis]) ++axis;                       // the last end is half
+                pos = p.pos[(static_cast<size_t>(axis) * p.batch + b) * p.max_q + row + t];
+            }
+            cs[t * half + pr] = turn(pos, p.inv_freq[pr]);
+        }
+        __syncthreads();
+        if (!kv) {
+            const T* q = static_cast<const T*>(p.q);
+            T* out = static_cast<T*>(p.q_out);
+            const uint32_t total = cnt * nh * row_items;
+            for (uint32_t i = threadIdx.x; i < total; i += kRopeThreads) {
+                const uint32_t t = i / (nh * row_items), r = i % (nh * row_items);
+                const uint32_t h = h0 + r / row_items, it = r % row_items;
+                const Item<VEC> x(it, p.rotary, p.interleaved);
+                const T* src = q + (row0 + row + t) * p.q_pitch + static_cast<size_t>(h) * D;
+                T* dst = out + ((row0 + row + t) * p.hq + h) * D;
+                Vec<T, VEC> u = load_vec<T, VEC>(src + x.e0), w;
+                const bool two = x.e1 < D;
+                if (two) w = load_vec<T, VEC>(src + x.e1);
+                if (x.turned) rotate<T, VEC>(u, w, cs + t * half + it * VEC, p.interleaved);
+                store_vec<T, VEC>(dst + x.e0, u);
+                if (two) store_vec<T, VEC>(dst + x.e1, w);
+            }
+            continue;
+        }
+        const T* v = static_cast<const T*>(p.v);
+        const uint32_t v_items = static_cast<uint32_t>(slot_elems / VEC);
+        for (uint32_t i = threadIdx.x; i < cnt * v_items; i += kRopeThreads) {
+            const uint32_t t = i / v_items, e = (i % v_items) * VEC;
+            store_vec<T, VEC>(vslots + (t0 - base + t) * slot_elems + e,
+                              load_vec<T, VEC>(v + (row0 + row + t) * p.v_pitch + e));
+        }
+        const T* k = static_cast<const T*>(p.k);
+        for (uint32_t i = threadIdx.x; i < groups * k_items; i += kRopeThreads) {
+            const uint32_t g = i / k_items, h = (i % k_items) / row_items, it = i % row_items;
+            const Item<VEC> x(it, p.rotary, p.interleaved);
+            const bool two = x.e1 < D;
+            for (uint32_t t = g; t < cnt; t += groups) {
+                const T* src = k + (row0 + row + t) * p.k_pitch + static_cast<size_t>(h) * D;
+                T* dst = kslots + (t0 - base + t) * slot_elems + static_cast<size_t>(h) * D;
+                Vec<T, VEC> u = load_vec<T, VEC>(src + x.e0), w;
+                if (two) w = load_vec<T, VEC>(src + x.e1);
+                if (x.turned) rotate<T, VEC>(u, w, cs + t * half + it * VEC, p.interleaved);
+                store_vec<T, VEC>(dst + x.e0, u);
+                if (two) store_vec<T, VEC>(dst + x.e1, w);
+            }
+        }
+    }
+    if (!kv || p.summary == nullptr) return;
+
+    // The block's K is in the pool now, old slots and new ones: this CTA's own
+    // writes are visible to it after the barrier.
+    __syncthreads();
+    const uint32_t filled = min(p.T, static_cast<uint32_t>(ctx) - base);
+    T* bounds = reinterpret_cast<T*>(p.summary + static_cast<size_t>(id) * p.summary_stride) +
+                static_cast<size_t>(p.layer) * 2 * slot_elems;
+    for (uint32_t i0 = 0; i0 < groups * k_items; i0 += kRopeThreads) {
+        const uint32_t i = i0 + threadIdx.x;
+        const bool live = i < groups * k_items;
+        const uint32_t g = i / k_items, h = (i % k_items) / row_items, it = i % row_items;
+        const Item<VEC> x(it, p.rotary, p.interleaved);
+        const bool two = x.e1 < D;
+        Vec<T, VEC> lo0, hi0, lo1, hi1;
+        start_range(lo0, hi0);
+        start_range(lo1, hi1);
+        if (live) {
+            for (uint32_t s = g; s < filled; s += groups) {
+                const T* src = kslots + s * slot_elems + static_cast<size_t>(h) * D;
+                const Vec<T, VEC> u = load_vec<T, VEC>(src + x.e0);
+                widen(lo0, hi0, u, u);
+                if (two) {
+                    const Vec<T, VEC> w = load_vec<T, VEC>(src + x.e1);
+                    widen(lo1, hi1, w, w);
+                }
+            }
+        }
+        if (groups > 1) {
+            part[threadIdx.x][0] = lo0;
+            part[threadIdx.x][1] = hi0;
+            part[threadIdx.x][2] = lo1;
+            part[threadIdx.x][3] = hi1;
+            __syncthreads();
+            if (live && g == 0) {
+                for (uint32_t o = 1; o < groups; ++o) {
+                    widen(lo0, hi0, part[o * k_items + i][0], part[o * k_items + i][1]);
+                    widen(lo1, hi1, part[o * k_items + i][2], part[o * k_items + i][3]);
+                }
+            }
+        }
+        if (live && g == 0) {
+            T* dst = bounds + static_cast<size_t>(h) * 2 * D;
+            store_vec<T, VEC>(dst + x.e0, lo0);
+            store_vec<T, VEC>(dst + D + x.e0, hi0);
+            if (two) {
+                store_vec<T, VEC>(dst + x.e1, lo1);
+                store_vec<T, VEC>(dst + D + x.e1, hi1);
+            }
+        }
+    }
+}
+
+template <typename T>
+int launch_rope(const RopeParams& p, bool vec, dim3 grid, cudaStream_t st) {
+    if (vec)
+        return launch_dependent("launch rope_append", rope_append_kernel<T, 16 / sizeof(T)>, grid, kRopeThreads, 0, 1,
+                                st, p);
+    return launch_dependent("launch rope_append", rope_append_kernel<T, 1>, grid, kRopeThreads, 0, 1, st, p);
+}
+
+}  // namespace
+
+}  // namespace qvp
+
+using namespace qvp;
+
+extern "C" int qvp_rope_append(const qvp_rope_append_args* args, qvp_stream_t stream) {
+    if (args == nullptr) return fail(QVP_ERR_INVALID, "null argument");
+    const qvp_rope_append_args& a = *args;
+    const qvp_block_shape& sh = a.shape;
+    int rc = check_shape(sh, a.dtype, a.layer);
+    if (rc != QVP_OK) return rc;
+    const uint32_t elem = sh.bytes_per_element, D = sh.head_dim;
+    if (a.num_query_heads % sh.num_kv_heads != 0)
+        return fail(QVP_ERR_INVALID, "num_query_heads %u is not a multiple of num_kv_heads %u", a.num_query_heads,
+                    sh.num_kv_heads);
+    if (a.num_query_heads > 65535u) return fail(QVP_ERR_UNSUPPORTED, "more than 65535 query heads");
+    if (a.rotary_dim % 2 != 0 || a.rotary_dim > D)
+        return fail(QVP_ERR_INVALID, "rotary_dim %u is odd or above head_dim %u", a.rotary_dim, D);
+    if (a.rotary_dim > 0 && a.rope_positions != nullptr) {
+        if (a.rope_axes == 0 || a.rope_axes > QVP_ROPE_MAX_AXES)
+            return fail(QVP_ERR_INVALID, "rope_axes %u is not in 1 .. %d", a.rope_axes, QVP_ROPE_MAX_AXES);
+        uint64_t pairs = 0;
+        for (uint32_t i = 0; i < a.rope_axes; ++i) pairs += a.rope_sections[i];
+        if (pairs != a.rotary_dim / 2)
+            return fail(QVP_ERR_INVALID, "rope_sections do not add up to rotary_dim / 2");
+    }
+    if (a.batch == 0) return QVP_OK;
+    rc = check_pool("pool", a.pool, a.block_stride, qvp_block_bytes(&sh), elem, a.num_blocks);
+    if (rc != QVP_OK) return rc;
+    rc = check_tables(a.block_tables, a.context_lens, a.max_blocks_per_seq, a.batch);
+    if (rc != QVP_OK) return rc;
+    if (a.query_lens == nullptr || a.key == nullptr || a.value == nullptr)
+        return fail(QVP_ERR_INVALID, "null length, key or value pointer");
+    if (a.max_query_len == 0 || a.max_query_len > 0x7fffffffu)
+        return fail(QVP_ERR_INVALID, "max_query_len %u is zero or above 2^31 - 1", a.max_query_len);
+    if (a.rotary_dim > 0 && a.inv_freq == nullptr) return fail(QVP_ERR_INVALID, "null inv_freq");
+    const size_t q_row = static_cast<size_t>(a.num_query_heads) * D, kv_row = static_cast<size_t>(sh.num_kv_heads) * D;
+    const size_t q_pitch = a.query_pitch != 0 ? a.query_pitch : q_row;
+    const size_t k_pitch = a.key_pitch != 0 ? a.key_pitch : kv_row;
+    const size_t v_pitch = a.value_pitch != 0 ? a.value_pitch : kv_row;
+    if (k_pitch < kv_row || v_pitch < kv_row) return fail(QVP_ERR_INVALID, "key or value pitch below a token's row");
+    if (!aligned_to(a.key, elem) || !aligned_to(a.value, elem))
+        return fail(QVP_ERR_INVALID, "key or value is not element-aligned");
+    if (a.num_query_heads > 0) {
+        if (a.query == nullptr || a.query_out == nullptr) return fail(QVP_ERR_INVALID, "null query or query_out");
+        if (q_pitch < q_row) return fail(QVP_ERR_INVALID, "query pitch below a token's row");
+        if (a.query_out == a.query && q_pitch != q_row)
+            return fail(QVP_ERR_INVALID, "query_out is dense: it cannot be a query with a pitch");
+        if (!aligned_to(a.query, elem) || !aligned_to(a.query_out, elem))
+            return fail(QVP_ERR_INVALID, "query or query_out is not element-aligned");
+    }
+    qvp_block_shape ss;
+    qvp_summary_shape(&sh, &ss);
+    if (a.summary != nullptr) {
+        rc = check_pool("summary pool", a.summary, a.summary_stride, qvp_block_bytes(&ss), elem, a.num_blocks);
+        if (rc != QVP_OK) return rc;
+    }
+
+    RopeParams p;
+    p.pool = static_cast<uint8_t*>(a.pool);
+    p.block_stride = a.block_stride;
+    p.tables = a.block_tables;
+    p.ctx = a.context_lens;
+    p.qlen = a.query_lens;
+    p.q = a.query;
+    p.k = a.key;
+    p.v = a.value;
+    p.q_out = a.query_out;
+    p.q_pitch = q_pitch;
+    p.k_pitch = k_pitch;
+    p.v_pitch = v_pitch;
+    p.inv_freq = a.inv_freq;
+    p.pos = a.rotary_dim > 0 ? a.rope_positions : nullptr;
+    p.summary = static_cast<uint8_t*>(a.summary);
+    p.summary_stride = a.summary_stride;
+    p.err = a.error_word;
+    p.num_blocks = a.num_blocks;
+    p.pitch = a.max_blocks_per_seq;
+    p.capacity = token_capacity(a.max_blocks_per_seq, sh.tokens_per_block);
+    p.T = sh.tokens_per_block;
+    p.layer = a.layer;
+    p.hq = a.num_query_heads;
+    p.hkv = sh.num_kv_heads;
+    p.D = D;
+    p.batch = a.batch;
+    p.max_q = a.max_query_len;
+    p.rotary = a.rotary_dim;
+    p.interleaved = a.rotary_interleaved != 0;
+    uint32_t end = 0;
+    for (uint32_t i = 0; i < QVP_ROPE_MAX_AXES; ++i) {
+        end += p.pos != nullptr && i < a.rope_axes ? a.rope_sections[i] : 0;
+        p.section_end[i] = end;
+    }
+    // n tokens that start anywhere in a block touch at most this many blocks
+    p.units = static_cast<uint32_t>((static_cast<uint64_t>(a.max_query_len) + p.T - 2) / p.T + 1);
+    p.units = p.units < a.max_blocks_per_seq ? p.units : a.max_blocks_per_seq;
+    if (static_cast<uint64_t>(p.units) * a.batch > 0x7fffffffu)
+        return fail(QVP_ERR_UNSUPPORTED, "more than 2^31 blocks in one call");
+    p.heads_per_cta = 8;
+    const uint32_t groups = a.num_query_heads > 0 ? ceil_div(a.num_query_heads, p.heads_per_cta) : 0;
+    const dim3 grid(p.units * a.batch, 1 + groups);
+
+    const uint32_t V = 16 / elem;
+    const bool vec = D % (2 * V) == 0 && a.rotary_dim % (2 * V) == 0 && aligned_to(a.pool, 16) &&
+                     a.block_stride % 16 == 0 && aligned_to(a.key, 16) && aligned_to(a.value, 16) &&
+                     k_pitch % V == 0 && v_pitch % V == 0 &&
+                     (a.num_query_heads == 0 ||
+                      (aligned_to(a.query, 16) && aligned_to(a.query_out, 16) && q_pitch % V == 0)) &&
+                     (a.summary == nullptr || (aligned_to(a.summary, 16) && a.summary_stride % 16 == 0));
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return a.dtype == QVP_DTYPE_F32 ? launch_rope<float>(p, vec, grid, st) : launch_rope<__nv_bfloat16>(p, vec, grid, st);
+}

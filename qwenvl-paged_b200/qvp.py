@@ -98,6 +98,110 @@ class PrefillArgs(C.Structure):
     ]
 
 
+ROPE_MAX_AXES = 4
+
+
+class RopeAppendArgs(C.Structure):
+    _fields_ = [
+        ("pool", C.c_void_p),
+        ("block_stride", C.c_size_t),
+        ("num_blocks", C.c_uint32),
+        ("shape", BlockShape),
+        ("dtype", C.c_int32),
+        ("layer", C.c_uint32),
+        ("num_query_heads", C.c_uint32),
+        ("batch", C.c_uint32),
+        ("max_blocks_per_seq", C.c_uint32),
+        ("max_query_len", C.c_uint32),
+        ("block_tables", C.c_void_p),
+        ("context_lens", C.c_void_p),
+        ("query_lens", C.c_void_p),
+        ("query", C.c_void_p),
+        ("key", C.c_void_p),
+        ("value", C.c_void_p),
+        ("query_out", C.c_void_p),
+        ("query_pitch", C.c_size_t),
+        ("key_pitch", C.c_size_t),
+        ("value_pitch", C.c_size_t),
+        ("rotary_dim", C.c_uint32),
+        ("rotary_interleaved", C.c_uint32),
+        ("inv_freq", C.c_void_p),
+        ("rope_positions", C.c_void_p),
+        ("rope_axes", C.c_uint32),
+        ("rope_sections", C.c_uint32 * ROPE_MAX_AXES),
+        ("summary", C.c_void_p),
+        ("summary_stride", C.c_size_t),
+        ("error_word", C.c_void_p),
+    ]
+
+
+class SummarizeArgs(C.Structure):
+    _fields_ = [
+        ("pool", C.c_void_p),
+        ("block_stride", C.c_size_t),
+        ("num_blocks", C.c_uint32),
+        ("shape", BlockShape),
+        ("dtype", C.c_int32),
+        ("layer", C.c_uint32),
+        ("batch", C.c_uint32),
+        ("max_blocks_per_seq", C.c_uint32),
+        ("max_context_len", C.c_uint32),
+        ("block_tables", C.c_void_p),
+        ("context_lens", C.c_void_p),
+        ("first_tokens", C.c_void_p),
+        ("summary", C.c_void_p),
+        ("summary_stride", C.c_size_t),
+        ("error_word", C.c_void_p),
+    ]
+
+
+class SelectArgs(C.Structure):
+    _fields_ = [
+        ("summary", C.c_void_p),
+        ("summary_stride", C.c_size_t),
+        ("num_blocks", C.c_uint32),
+        ("shape", BlockShape),
+        ("dtype", C.c_int32),
+        ("layer", C.c_uint32),
+        ("num_query_heads", C.c_uint32),
+        ("batch", C.c_uint32),
+        ("max_blocks_per_seq", C.c_uint32),
+        ("max_context_len", C.c_uint32),
+        ("block_tables", C.c_void_p),
+        ("context_lens", C.c_void_p),
+        ("query", C.c_void_p),
+        ("query_pitch", C.c_size_t),
+        ("max_selected", C.c_uint32),
+        ("sink_blocks", C.c_uint32),
+        ("recent_blocks", C.c_uint32),
+        ("selected", C.c_void_p),
+        ("error_word", C.c_void_p),
+    ]
+
+
+class DecodeSelectedArgs(C.Structure):
+    _fields_ = [
+        ("pool", C.c_void_p),
+        ("block_stride", C.c_size_t),
+        ("num_blocks", C.c_uint32),
+        ("shape", BlockShape),
+        ("dtype", C.c_int32),
+        ("layer", C.c_uint32),
+        ("num_query_heads", C.c_uint32),
+        ("scale", C.c_float),
+        ("batch", C.c_uint32),
+        ("max_blocks_per_seq", C.c_uint32),
+        ("block_tables", C.c_void_p),
+        ("context_lens", C.c_void_p),
+        ("query", C.c_void_p),
+        ("query_pitch", C.c_size_t),
+        ("selected", C.c_void_p),
+        ("max_selected", C.c_uint32),
+        ("out", C.c_void_p),
+        ("error_word", C.c_void_p),
+    ]
+
+
 class Shard(C.Structure):
     _fields_ = [("shard", C.c_uint32), ("num_shards", C.c_uint32), ("device", C.c_int)]
 
@@ -150,6 +254,11 @@ def _load() -> C.CDLL:
         "qvp_compress_blocks": (C.c_int, [vp, sz, u32, sz, vp, vp, u32, vp, sz, vp, sz, u32, vp, vp, vp]),
         "qvp_decompress_blocks": (C.c_int, [vp, sz, u32, sz, vp, vp, u32, vp, sz, vp, sz, u32, vp, vp, vp]),
         "qvp_kv_append": (C.c_int, [vp, sz, u32, P(BlockShape), u32, u32, u32, vp, vp, vp, vp, vp, vp]),
+        "qvp_summary_shape": (C.c_int, [P(BlockShape), P(BlockShape)]),
+        "qvp_rope_append": (C.c_int, [P(RopeAppendArgs), vp]),
+        "qvp_summarize_blocks": (C.c_int, [P(SummarizeArgs), vp]),
+        "qvp_select_blocks": (C.c_int, [P(SelectArgs), vp]),
+        "qvp_decode_selected": (C.c_int, [P(DecodeSelectedArgs), vp]),
         "qvp_shard_gather_bytes": (C.c_int, [P(ShardDecodeArgs), P(sz)]),
         "qvp_shard_decode": (C.c_int, [P(ShardDecodeArgs), vp]),
         "qvp_shard_reassemble": (C.c_int, [vp, vp, u32, u32, u32, u32, u32, vp]),
@@ -179,7 +288,8 @@ EXPORTED = [
     "qvp_pool_device", "qvp_pool_write", "qvp_pool_read", "qvp_decode_workspace_size",
     "qvp_decode_plan", "qvp_decode", "qvp_decode_noalloc", "qvp_prefill", "qvp_copy_blocks", "qvp_gather_blocks", "qvp_scatter_blocks",
     "qvp_swap_slot_bytes", "qvp_compress_blocks", "qvp_decompress_blocks", "qvp_fetch_host",
-    "qvp_kv_append", "qvp_shard_gather_bytes", "qvp_shard_decode", "qvp_shard_reassemble",
+    "qvp_kv_append", "qvp_summary_shape", "qvp_rope_append", "qvp_summarize_blocks", "qvp_select_blocks",
+    "qvp_decode_selected", "qvp_shard_gather_bytes", "qvp_shard_decode", "qvp_shard_reassemble",
     "qvp_nccl_unique_id", "qvp_nccl_comm_init", "qvp_nccl_comm_destroy",
     "qvp_peer_group_create", "qvp_peer_group_open", "qvp_peer_group_destroy", "qvp_peer_group_output",
     "qvp_shard_decode_peer",
@@ -261,6 +371,72 @@ def decode_plan(args: DecodeArgs):
 def decode(args: DecodeArgs, stream: int = 0) -> int:
     """Enqueues one batched decode; returns the status (does not raise)."""
     return lib.qvp_decode(C.byref(args), stream or None)
+
+
+def summary_shape(shape: BlockShape) -> BlockShape:
+    """The block shape of the summary pool of a cache with blocks of `shape`."""
+    out = BlockShape()
+    check(lib.qvp_summary_shape(C.byref(shape), C.byref(out)), "qvp_summary_shape")
+    return out
+
+
+def rope_append_args(*, pool, block_stride, num_blocks, shape, dtype, layer, num_query_heads, batch,
+                     max_blocks_per_seq, max_query_len, block_tables, context_lens, query_lens, key, value,
+                     query=0, query_out=0, query_pitch=0, key_pitch=0, value_pitch=0, rotary_dim=0,
+                     rotary_interleaved=0, inv_freq=0, rope_positions=0, rope_sections=(), summary=0,
+                     summary_stride=0, error_word=0) -> RopeAppendArgs:
+    """`rope_sections` holds the pairs of each axis (its length is rope_axes)."""
+    sections = list(rope_sections)
+    if len(sections) > ROPE_MAX_AXES:
+        raise ValueError(f"more than {ROPE_MAX_AXES} rotary axes")
+    return RopeAppendArgs(pool, block_stride, num_blocks, shape, dtype, layer, num_query_heads, batch,
+                          max_blocks_per_seq, max_query_len, block_tables, context_lens, query_lens, query or None,
+                          key, value, query_out or None, query_pitch, key_pitch, value_pitch, rotary_dim,
+                          rotary_interleaved, inv_freq or None, rope_positions or None, len(sections),
+                          (C.c_uint32 * ROPE_MAX_AXES)(*sections), summary or None, summary_stride,
+                          error_word or None)
+
+
+def summarize_args(*, pool, block_stride, num_blocks, shape, dtype, layer, batch, max_blocks_per_seq,
+                   max_context_len, block_tables, context_lens, summary, summary_stride, first_tokens=0,
+                   error_word=0) -> SummarizeArgs:
+    return SummarizeArgs(pool, block_stride, num_blocks, shape, dtype, layer, batch, max_blocks_per_seq,
+                         max_context_len, block_tables, context_lens, first_tokens or None, summary, summary_stride,
+                         error_word or None)
+
+
+def select_args(*, summary, summary_stride, num_blocks, shape, dtype, layer, num_query_heads, batch,
+                max_blocks_per_seq, max_context_len, block_tables, context_lens, query, max_selected, selected,
+                query_pitch=0, sink_blocks=0, recent_blocks=0, error_word=0) -> SelectArgs:
+    return SelectArgs(summary, summary_stride, num_blocks, shape, dtype, layer, num_query_heads, batch,
+                      max_blocks_per_seq, max_context_len, block_tables, context_lens, query, query_pitch,
+                      max_selected, sink_blocks, recent_blocks, selected, error_word or None)
+
+
+def decode_selected_args(*, pool, block_stride, num_blocks, shape, dtype, layer, num_query_heads, scale, batch,
+                         max_blocks_per_seq, block_tables, context_lens, query, selected, max_selected, out,
+                         query_pitch=0, error_word=0) -> DecodeSelectedArgs:
+    return DecodeSelectedArgs(pool, block_stride, num_blocks, shape, dtype, layer, num_query_heads, scale, batch,
+                              max_blocks_per_seq, block_tables, context_lens, query, query_pitch, selected,
+                              max_selected, out, error_word or None)
+
+
+# The sparse-attention calls enqueue one operator each and return the status
+# (they do not raise), as decode() does.
+def rope_append(args: RopeAppendArgs, stream: int = 0) -> int:
+    return lib.qvp_rope_append(C.byref(args), stream or None)
+
+
+def summarize_blocks(args: SummarizeArgs, stream: int = 0) -> int:
+    return lib.qvp_summarize_blocks(C.byref(args), stream or None)
+
+
+def select_blocks(args: SelectArgs, stream: int = 0) -> int:
+    return lib.qvp_select_blocks(C.byref(args), stream or None)
+
+
+def decode_selected(args: DecodeSelectedArgs, stream: int = 0) -> int:
+    return lib.qvp_decode_selected(C.byref(args), stream or None)
 
 
 def nccl_unique_id() -> bytes:
