@@ -1300,11 +1300,23 @@ int encode_pool_map_box(const void* pool, uint32_t num_blocks, const qvp_block_s
         *map = cached;
         return QVP_OK;
     }
+    qvp_block_shape sixteen = shape;  // the dense kernels' blocks have 16 tokens
+    sixteen.tokens_per_block = 16;
+    const int rc = make_pool_map(pool, num_blocks, sixteen, hh, rows, halves, map);
+    if (rc != QVP_OK) return rc;
+    last = key;
+    cached = *map;
+    return QVP_OK;
+}
+
+int make_pool_map(const void* pool, uint32_t num_blocks, const qvp_block_shape& shape, uint32_t hh, uint32_t rows,
+                  uint32_t halves, CUtensorMap* map) {
     auto encode = get_encode_fn();
     if (encode == nullptr) return fail(QVP_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
     const uint32_t D = shape.head_dim;
     const uint32_t H = shape.num_kv_heads;
-    cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(num_blocks) * shape.num_layers * 2 * 16, H, D / 64};
+    cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(num_blocks) * shape.num_layers * 2 * shape.tokens_per_block, H,
+                          D / 64};
     cuuint64_t strides[3] = {static_cast<cuuint64_t>(H) * D * 2, static_cast<cuuint64_t>(D) * 2, 128};
     cuuint32_t box[4] = {64, rows, hh, halves};
     cuuint32_t estr[4] = {1, 1, 1, 1};
@@ -1312,8 +1324,6 @@ int encode_pool_map_box(const void* pool, uint32_t num_blocks, const qvp_block_s
                         estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(QVP_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", int(r));
-    last = key;
-    cached = *map;
     return QVP_OK;
 }
 

@@ -11,6 +11,11 @@
 #include "attention_tile.cuh"
 #include "sparse_common.cuh"
 
+#include <cooperative_groups.h>
+#include <cuda.h>
+
+namespace cg = cooperative_groups;
+
 namespace qvp {
 
 namespace {
@@ -28,10 +33,347 @@ struct SelectedParams {
     uint32_t num_blocks;
     uint32_t pitch;
     uint32_t capacity;
-    uint32_t T, layer, hq, hkv, D, group;
+    uint32_t T, layer, num_layers, hq, hkv, D, group;
     uint32_t keep;
+    uint32_t cluster;  // CTAs that share a (sequence, kv head)
     float scale_log2;  // scale * log2(e): the softmax is computed in powers of two
 };
+
+// ---------------------------------------------------------------------------
+// bf16, head_dim 64 or 128, blocks of a multiple of 16 tokens, unpadded.
+//
+// The work of a (sequence, kv head) is a list of 16-token pieces, dealt round
+// robin to the warps of a cluster of CTAs. Each warp streams its own pieces
+// with TMA into a ring of its own (K and V of a piece: 4 * head_dim * 16
+// bytes) and needs no other warp until the end, so there is no producer warp
+// and no barrier in the loop. Q K^T and P V run on mma.sync m16n8k16 with the
+// group padded to 16 rows; they are a small part of the time (the kernel is
+// bound by HBM), and tcgen05's 128-row tiles would be 6 % full.
+//
+// A group of at most 8 heads leaves the upper 8 rows of the tile free: the
+// weights' rounding remainders go there (P = hi + lo, both bf16), so P V
+// loses 2^-16 of a weight instead of 2^-8 at no cost. Larger groups multiply
+// bf16 weights, as the dense decode does.
+//
+// At the end the warps' partial results are joined through distributed shared
+// memory: no workspace, no second kernel, and a fixed order.
+// ---------------------------------------------------------------------------
+
+constexpr int kTileWarps = 4;
+constexpr int kTileThreads = kTileWarps * 32;
+constexpr uint32_t kTileMaxCluster = 8;
+
+template <int D, int STAGES>
+struct TileShape {
+    static constexpr uint32_t kPiece = 2 * 16 * D * 2;               // K and V of 16 tokens of one head
+    static constexpr uint32_t kRing = STAGES * kPiece;               // one warp's
+    static constexpr uint32_t kBars = kTileWarps * kRing;            // offset of the barriers
+    static constexpr uint32_t kStats = kBars + kTileWarps * STAGES * 8;  // m, l of 16 rows per warp, tokens seen
+    static constexpr uint32_t kSmem = kStats + kTileWarps * (32 * 4 + 16) + 1024;
+    static_assert(kRing >= 16 * D * 4, "a warp's partial output takes the place of its ring");
+};
+
+// One piece: online-softmax update of the 16 rows of `st`. `valid` of its
+// tokens are below the context. Where PAIR, rows 8..15 carry the remainders
+// of the weights of rows 0..7 (st.m1, st.l1 unused).
+template <int D, bool PAIR, bool SPLIT>
+__device__ __forceinline__ void attend_piece(WarpState<D>& st, const uint32_t (&qa)[D / 16][4], uint32_t piece,
+                                             int valid, float scale_log2, int lane) {
+    // K and V of a 64-column half: K | V adjacent in one box, or all K before all V
+    constexpr uint32_t kHalf = SPLIT ? 2048u : 4096u;
+    constexpr uint32_t kV = SPLIT ? static_cast<uint32_t>(D / 64) * 2048u : 2048u;
+    const int c = lane & 3;
+    const int mi = lane >> 3;
+    const int li = lane & 7;
+    float s[2][4];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) s[a][0] = s[a][1] = s[a][2] = s[a][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        const int chunk = ((ks & 3) << 1) + (mi & 1);
+        const int t = ((mi >> 1) << 3) + li;
+        uint32_t r0, r1, r2, r3;
+        ldmatrix_x4(box_addr(piece + (ks >> 2) * kHalf, 0, t, chunk), r0, r1, r2, r3);
+        mma_bf16_16816(s[0], qa[ks], r0, r1);
+        mma_bf16_16816(s[1], qa[ks], r2, r3);
+    }
+    constexpr int kRows = PAIR ? 1 : 2;
+    uint32_t pa[4];
+    float corr[2] = {1.f, 1.f};
+    bool grew = false;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        float x[4];  // this lane's four scores of row g + 8 r: keys 2c, 2c + 1, 8 + 2c, 9 + 2c
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int tok = (e >> 1) * 8 + c * 2 + (e & 1);
+            x[e] = tok < valid ? s[e >> 1][2 * r + (e & 1)] * scale_log2 : -INFINITY;
+        }
+        float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        float& m = r == 0 ? st.m0 : st.m1;
+        float& l = r == 0 ? st.l0 : st.l1;
+        const float m_new = fmaxf(m, top);
+        const float m_ref = m_new == -INFINITY ? 0.f : m_new;  // nothing above -inf yet: weights are 0, not NaN
+        grew |= m_new > m;
+        corr[r] = exp2f(m - m_ref);
+        m = m_new;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = exp2f(x[e] - m_ref);
+        l = l * corr[r] + ((x[0] + x[1]) + (x[2] + x[3]));
+        pa[r] = pack_bf16x2(x[0], x[1]);
+        pa[r + 2] = pack_bf16x2(x[2], x[3]);
+        if constexpr (PAIR) {
+            auto low = [](float u, float w, uint32_t hi) {
+                const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&hi);
+                return pack_bf16x2(u - __low2float(h), w - __high2float(h));
+            };
+            pa[1] = low(x[0], x[1], pa[0]);
+            pa[3] = low(x[2], x[3], pa[2]);
+        }
+    }
+    if (__any_sync(0xffffffffu, grew)) {
+        const float c0 = corr[0], c1 = PAIR ? corr[0] : corr[1];
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+            st.o[n][0] *= c0;
+            st.o[n][1] *= c0;
+            st.o[n][2] *= c1;
+            st.o[n][3] *= c1;
+        }
+    }
+#pragma unroll
+    for (int np = 0; np < D / 16; ++np) {
+        const int chunk = ((np & 3) << 1) + (mi >> 1);
+        const int t = ((mi & 1) << 3) + li;
+        uint32_t v0, v1, v2, v3;
+        ldmatrix_x4_trans(box_addr(piece + (np >> 2) * kHalf + kV, 0, t, chunk), v0, v1, v2, v3);
+        if (valid < 16) {  // V slots past the context may hold anything, NaN included
+            v0 = mask_pair(v0, c * 2, valid);
+            v2 = mask_pair(v2, c * 2, valid);
+            v1 = mask_pair(v1, 8 + c * 2, valid);
+            v3 = mask_pair(v3, 8 + c * 2, valid);
+        }
+        mma_bf16_16816(st.o[2 * np], pa, v0, v1);
+        mma_bf16_16816(st.o[2 * np + 1], pa, v2, v3);
+    }
+}
+
+// grid (segments * cluster, chunks of 16 heads of a group)
+template <int D, int STAGES, bool PAIR, bool SPLIT>
+__global__ void __launch_bounds__(kTileThreads, 2)
+    decode_selected_tile(const __grid_constant__ CUtensorMap tmap, const SelectedParams p) {
+    using S = TileShape<D, STAGES>;
+    constexpr int NT = D / 8;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~static_cast<uintptr_t>(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = smem_u32(smem + warp * S::kRing);
+    const uint32_t bars = smem_u32(smem + S::kBars) + warp * STAGES * 8;
+    if (lane == 0) {
+        prefetch_tensormap(&tmap);
+        for (int s = 0; s < STAGES; ++s) mbar_init(bars + 8 * s, 1);
+        mbar_fence_init();
+    }
+    __syncwarp();
+    wait_for_previous_kernel();
+    allow_next_kernel();
+
+    const uint32_t cluster = p.cluster;
+    const uint32_t rank = blockIdx.x % cluster, seg = blockIdx.x / cluster;
+    const uint32_t b = seg / p.hkv, head = seg % p.hkv;
+    const int G = static_cast<int>(min(p.group - blockIdx.y * 16, 16u));  // heads of this chunk
+    const size_t h0 = static_cast<size_t>(head) * p.group + blockIdx.y * 16;
+    const int ctx = p.ctx[b];
+    if (ctx < 0 || static_cast<uint32_t>(ctx) > p.capacity) {  // the whole cluster
+        if (threadIdx.x == 0) record_error(p.err, kErrBadContext);
+        return;
+    }
+    const int32_t* list = p.selected + static_cast<size_t>(seg) * p.keep;
+    const int32_t* table = p.tables + static_cast<size_t>(b) * p.pitch;
+    const uint32_t per_block = p.T / 16;
+    const uint32_t nblk = (static_cast<uint32_t>(ctx) + p.T - 1) / p.T;
+    const uint64_t pieces = static_cast<uint64_t>(p.keep) * per_block;
+    const uint32_t workers = cluster * kTileWarps, worker = rank * kTileWarps + warp;
+
+    uint32_t qa[D / 16][4];
+    {
+        const int g = lane >> 2, c = lane & 3;
+        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) + b * p.q_pitch + h0 * D;
+        const uint32_t* q_lo = reinterpret_cast<const uint32_t*>(q + g * D);
+        const uint32_t* q_hi = reinterpret_cast<const uint32_t*>(q + (g + 8) * D);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            const int k0 = (ks * 16 + c * 2) >> 1;
+            qa[ks][0] = g < G ? q_lo[k0] : 0u;
+            qa[ks][1] = g + 8 < G ? q_hi[k0] : 0u;
+            qa[ks][2] = g < G ? q_lo[k0 + 4] : 0u;
+            qa[ks][3] = g + 8 < G ? q_hi[k0 + 4] : 0u;
+        }
+    }
+    WarpState<D> st;
+    st.reset();
+    uint32_t seen = 0;                      // tokens attended by this warp
+    uint32_t issued = 0, used = 0;          // pieces of this warp
+    bool alive = true;
+    const uint64_t policy = l2_policy_evict_first();
+
+    // Lane l looks up the warp's l-th next piece: its K row in the pool and
+    // the tokens it has below the context (0: nothing to attend).
+    for (uint64_t base = worker; alive && base < pieces; base += static_cast<uint64_t>(workers) * 32) {
+        const uint64_t i = base + static_cast<uint64_t>(workers) * lane;
+        int valid = 0, krow = 0;
+        if (i < pieces && ctx > 0) {
+            const int32_t blk = list[i / per_block];
+            const uint32_t first = static_cast<uint32_t>(i % per_block) * 16;
+            if (blk >= 0) {
+                if (static_cast<uint32_t>(blk) >= nblk) {
+                    record_error(p.err, kErrBadBlockId);
+                } else {
+                    const int32_t id = table[blk];
+                    if (static_cast<uint32_t>(id) >= p.num_blocks)
+                        record_error(p.err, kErrBadBlockId);
+                    else {
+                        valid = max(0, min(16, ctx - static_cast<int>(static_cast<uint32_t>(blk) * p.T + first)));
+                        krow = static_cast<int>(((static_cast<uint32_t>(id) * p.num_layers + p.layer) * 2) * p.T + first);
+                    }
+                }
+            }
+        }
+        uint32_t to_issue = __ballot_sync(0xffffffffu, valid > 0), to_use = to_issue;
+        auto issue = [&]() {
+            const int from = __ffs(to_issue) - 1;
+            to_issue &= to_issue - 1;
+            const int row = __shfl_sync(0xffffffffu, krow, from);
+            if (lane == 0) {
+                const uint32_t slot = issued % STAGES;
+                const uint32_t dst = ring + slot * S::kPiece, bar = bars + 8 * slot;
+                mbar_arrive_expect_tx(bar, S::kPiece);
+                tma_load_4d(dst, &tmap, bar, 0, row, static_cast<int>(head), 0, policy);
+                if constexpr (SPLIT)
+                    tma_load_4d(dst + S::kPiece / 2, &tmap, bar, 0, row + static_cast<int>(p.T), static_cast<int>(head),
+                                0, policy);
+            }
+            ++issued;
+        };
+        while (to_issue != 0 && issued - used < STAGES) issue();
+        while (to_use != 0) {
+            const int from = __ffs(to_use) - 1;
+            to_use &= to_use - 1;
+            const int n = __shfl_sync(0xffffffffu, valid, from);
+            const uint32_t slot = used % STAGES;
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * slot, (used / STAGES) & 1u))) {
+                if (lane == 0) record_error(p.err, kErrWaitTimeout);
+                alive = false;
+                break;
+            }
+            attend_piece<D, PAIR, SPLIT>(st, qa, ring + slot * S::kPiece, n, p.scale_log2, lane);
+            seen += n;
+            ++used;
+            __syncwarp();  // every lane has read the slot before it is filled again
+            if (to_issue != 0) issue();
+        }
+    }
+    // after a wait that ran out, no copy may still be landing below
+    for (; used < issued; ++used) mbar_wait_bounded(bars + 8 * (used % STAGES), (used / STAGES) & 1u);
+
+    // This warp's partial result: 16 rows of D floats in its ring, m and l and
+    // the token count behind the rings.
+    st.l0 += __shfl_xor_sync(0xffffffffu, st.l0, 1);
+    st.l0 += __shfl_xor_sync(0xffffffffu, st.l0, 2);
+    st.l1 += __shfl_xor_sync(0xffffffffu, st.l1, 1);
+    st.l1 += __shfl_xor_sync(0xffffffffu, st.l1, 2);
+    __syncwarp();
+    {
+        const int g = lane >> 2, c = lane & 3;
+        float* part = reinterpret_cast<float*>(smem + warp * S::kRing);
+        float* stat = reinterpret_cast<float*>(smem + S::kStats) + warp * 36;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int col = n * 8 + c * 2;
+            if constexpr (PAIR) {
+                *reinterpret_cast<float2*>(part + g * D + col) =
+                    make_float2(st.o[n][0] + st.o[n][2], st.o[n][1] + st.o[n][3]);
+            } else {
+                *reinterpret_cast<float2*>(part + g * D + col) = make_float2(st.o[n][0], st.o[n][1]);
+                *reinterpret_cast<float2*>(part + (g + 8) * D + col) = make_float2(st.o[n][2], st.o[n][3]);
+            }
+        }
+        if (c == 0) {
+            stat[g] = st.m0;
+            stat[16 + g] = st.l0;
+            if constexpr (!PAIR) {
+                stat[8 + g] = st.m1;
+                stat[24 + g] = st.l1;
+            }
+        }
+        if (lane == 0) reinterpret_cast<uint32_t*>(stat)[32] = seen;
+    }
+    auto barrier = [&]() {
+        if (cluster > 1)
+            cg::this_cluster().sync();
+        else
+            __syncthreads();
+    };
+    barrier();
+    // Each CTA of the cluster writes its share of the output, two elements a thread.
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + (static_cast<size_t>(b) * p.hq + h0) * D;
+    for (uint32_t i = rank * kTileThreads + threadIdx.x; i < static_cast<uint32_t>(G) * (D / 2);
+         i += cluster * kTileThreads) {
+        const uint32_t g = i / (D / 2), d = i % (D / 2) * 2;
+        float M = -INFINITY;
+        uint32_t any = 0;
+        for (uint32_t w = 0; w < workers; ++w) {
+            const uint8_t* at = cluster > 1 ? cg::this_cluster().map_shared_rank(smem, w / kTileWarps) : smem;
+            const float* stat = reinterpret_cast<const float*>(at + S::kStats) + (w % kTileWarps) * 36;
+            M = fmaxf(M, stat[g]);
+            any |= reinterpret_cast<const uint32_t*>(stat)[32];
+        }
+        float sum = 0.f, x = 0.f, y = 0.f;
+        for (uint32_t w = 0; w < workers; ++w) {
+            const uint8_t* at = cluster > 1 ? cg::this_cluster().map_shared_rank(smem, w / kTileWarps) : smem;
+            const float* stat = reinterpret_cast<const float*>(at + S::kStats) + (w % kTileWarps) * 36;
+            const float2 o = *reinterpret_cast<const float2*>(at + (w % kTileWarps) * S::kRing + (g * D + d) * 4);
+            const float m = stat[g];
+            // without a score above -inf the sums are 0, or NaN from a NaN score
+            const float weight = m == -INFINITY ? 1.f : exp2f(m - M);
+            sum += weight * stat[16 + g];
+            x += weight * o.x;
+            y += weight * o.y;
+        }
+        const float inv = any != 0 ? 1.f / sum : 0.f;
+        *reinterpret_cast<uint32_t*>(out + g * D + d) = any != 0 ? pack_bf16x2(x * inv, y * inv) : 0u;
+    }
+    // no CTA leaves while another may read its shared memory
+    barrier();
+}
+
+template <int D, int STAGES, bool PAIR, bool SPLIT>
+int launch_tile_t(const SelectedParams& p, const qvp_decode_selected_args& a, uint32_t segments, cudaStream_t st) {
+    using S = TileShape<D, STAGES>;
+    static std::atomic<std::uint64_t> attr_done{0};
+    auto kern = decode_selected_tile<D, STAGES, PAIR, SPLIT>;
+    int rc = set_smem_limit_once(attr_done, reinterpret_cast<const void*>(kern), S::kSmem,
+                                 "cudaFuncSetAttribute(decode_selected)");
+    if (rc != QVP_OK) return rc;
+    CUtensorMap map;
+    rc = make_pool_map(a.pool, a.num_blocks, a.shape, 1, SPLIT ? 16 : 32, D / 64, &map);
+    if (rc != QVP_OK) return rc;
+    const dim3 grid(segments * p.cluster, ceil_div(p.group, 16));
+    return launch_dependent("launch decode_selected", kern, grid, kTileThreads, S::kSmem, p.cluster, st, map, p);
+}
+
+template <int D, int STAGES>
+int launch_tile(const SelectedParams& p, const qvp_decode_selected_args& a, uint32_t segments, cudaStream_t st) {
+    const bool split = p.T != 16;
+    if (p.group <= 8)
+        return split ? launch_tile_t<D, STAGES, true, true>(p, a, segments, st)
+                     : launch_tile_t<D, STAGES, true, false>(p, a, segments, st);
+    return split ? launch_tile_t<D, STAGES, false, true>(p, a, segments, st)
+                 : launch_tile_t<D, STAGES, false, false>(p, a, segments, st);
+}
 
 // ---------------------------------------------------------------------------
 // Any type, block size, head_dim <= 256 and group. A warp takes 32 listed
@@ -347,6 +689,7 @@ extern "C" int qvp_decode_selected(const qvp_decode_selected_args* args, qvp_str
     p.capacity = token_capacity(a.max_blocks_per_seq, sh.tokens_per_block);
     p.T = sh.tokens_per_block;
     p.layer = a.layer;
+    p.num_layers = sh.num_layers;
     p.hq = a.num_query_heads;
     p.hkv = sh.num_kv_heads;
     p.D = sh.head_dim;
@@ -354,6 +697,21 @@ extern "C" int qvp_decode_selected(const qvp_decode_selected_args* args, qvp_str
     p.keep = a.max_selected;
     p.scale_log2 = a.scale * 1.4426950408889634f;  // log2(e)
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const uint64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
+    const bool tile = a.dtype == QVP_DTYPE_BF16 && (p.D == 64 || p.D == 128) && p.T % 16 == 0 &&
+                      a.block_stride == qvp_block_bytes(&sh) && aligned_to(a.pool, 16) && aligned_to(a.query, 4) &&
+                      q_pitch % 2 == 0 && aligned_to(a.out, 4) &&
+                      static_cast<uint64_t>(a.num_blocks) * sh.num_layers * 2 * p.T < (1ull << 31);
+    if (tile) {
+        const uint64_t pieces = static_cast<uint64_t>(p.keep) * (p.T / 16);
+        p.cluster = 1;
+        while (p.cluster < kTileMaxCluster && segments * p.cluster < 2 * sms && pieces > 2 * kTileWarps * p.cluster)
+            p.cluster *= 2;
+        if (segments * p.cluster > 0x7fffffffu) return fail(QVP_ERR_UNSUPPORTED, "more than 2^31 sequences and heads");
+        return p.D == 128 ? launch_tile<128, 3>(p, a, static_cast<uint32_t>(segments), st)
+                          : launch_tile<64, 6>(p, a, static_cast<uint32_t>(segments), st);
+    }
+    p.cluster = 1;
     return a.dtype == QVP_DTYPE_F32 ? launch_any<float>(p, a, static_cast<uint32_t>(segments), st)
                                     : launch_any<__nv_bfloat16>(p, a, static_cast<uint32_t>(segments), st);
 }

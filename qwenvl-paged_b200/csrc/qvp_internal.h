@@ -89,5 +89,9 @@ int encode_pool_map(const void* pool, uint32_t num_blocks, const qvp_block_shape
 // 32 = both) and `halves` 64-element halves of head_dim.
 int encode_pool_map_box(const void* pool, uint32_t num_blocks, const qvp_block_shape& shape, uint32_t hh,
                         uint32_t rows, uint32_t halves, CUtensorMap_st* map);
+// Encodes that view for blocks of any tokens_per_block T: token row of block
+// b, layer l, stream s, slot t is ((b*L + l)*2 + s)*T + t.
+int make_pool_map(const void* pool, uint32_t num_blocks, const qvp_block_shape& shape, uint32_t hh, uint32_t rows,
+                  uint32_t halves, CUtensorMap_st* map);
 
 }  // namespace qvp
