@@ -272,7 +272,7 @@ __device__ __forceinline__ void score_blocks(const SelectParams& p, const int32_
     const uint32_t lane = threadIdx.x & 31;
     for (uint32_t i = threadIdx.x >> 5; i < n; i += kSelWarps) {
         const int32_t id = table[first + i];
-        double s = -INFINITY;
+        double s = -kScoreLimit;
         if (static_cast<uint32_t>(id) >= p.num_blocks) {
             if (lane == 0) record_error(p.err, kErrBadBlockId);
         } else {
@@ -286,7 +286,89 @@ __device__ __forceinline__ void score_blocks(const SelectParams& p, const int32_
     }
 }
 
-template <typename T>
+// The same with 16-byte loads: LANES lanes per block, VECS vectors a lane, and
+// UNROLL blocks of every lane group in flight. A lane keeps the weights of its
+// columns in registers, and the UNROLL partial sums of a group are reduced
+// together: each exchange halves the sums a lane carries.
+template <typename T, int LANES, int VECS>
+__device__ __forceinline__ void score_blocks_vec(const SelectParams& p, const int32_t* table, uint32_t head,
+                                                 const double* weight, uint32_t first, uint32_t n, double* score) {
+    constexpr int V = 16 / sizeof(T);
+    constexpr int UNROLL = 8 / VECS;
+    constexpr uint32_t kGroups = 32 / LANES;           // blocks of a warp-wide load
+    constexpr uint32_t kStep = kGroups * UNROLL;       // blocks of a warp per step
+    static_assert(kStep <= 32, "a lane holds one id of a step");
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t col = lane % LANES, group = lane / LANES;
+    double w[VECS][V];
+    bool live[VECS];
+#pragma unroll
+    for (int j = 0; j < VECS; ++j) {
+        const uint32_t e = (col + j * LANES) * V;
+        live[j] = e < 2 * p.D;
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[j][i] = live[j] ? weight[e + i] : 0.0;
+    }
+    const T* rows = reinterpret_cast<const T*>(p.summary) + (static_cast<size_t>(p.layer) * p.hkv + head) * 2 * p.D +
+                    col * V;
+    const size_t stride = p.summary_stride / sizeof(T);
+    auto ids_of = [&](uint32_t base) -> int32_t {
+        const uint32_t i = base + lane;
+        return lane < kStep && i < n ? table[first + i] : 0;
+    };
+    int32_t next = ids_of(warp * kStep);
+    for (uint32_t base = warp * kStep; base < n; base += kSelWarps * kStep) {
+        const int32_t ids = next;
+        next = ids_of(base + kSelWarps * kStep);
+        const bool bad = static_cast<uint32_t>(ids) >= p.num_blocks;
+        if (bad) record_error(p.err, kErrBadBlockId);
+        Vec<T, V> x[UNROLL][VECS];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int32_t id = __shfl_sync(0xffffffffu, bad ? 0 : ids, u * kGroups + group);
+#pragma unroll
+            for (int j = 0; j < VECS; ++j)
+                if (live[j]) x[u][j] = load_vec<T, V>(rows + static_cast<size_t>(id) * stride + j * LANES * V);
+        }
+        double s[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            s[u] = 0.0;
+#pragma unroll
+            for (int j = 0; j < VECS; ++j)
+                if (live[j]) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) s[u] = fma(static_cast<double>(to_float<T>(x[u][j].v[i])), w[j][i], s[u]);
+                }
+        }
+        int live_sums = UNROLL;
+        uint32_t mine = 0;  // the sum this lane ends with
+#pragma unroll
+        for (int off = LANES / 2; off > 0; off >>= 1) {
+            if (live_sums > 1) {
+                live_sums >>= 1;
+#pragma unroll
+                for (int u = 0; u < UNROLL / 2; ++u) {
+                    if (u < live_sums) {
+                        const bool upper = lane & off;
+                        const double send = upper ? s[u] : s[u + live_sums];
+                        s[u] = (upper ? s[u + live_sums] : s[u]) + __shfl_xor_sync(0xffffffffu, send, off);
+                    }
+                }
+                mine = mine * 2 + ((lane & off) ? 1 : 0);
+            } else {
+                s[0] += __shfl_xor_sync(0xffffffffu, s[0], off);
+            }
+        }
+        constexpr uint32_t kSame = LANES / UNROLL;  // lanes that end with the same sum
+        const bool skip = __shfl_sync(0xffffffffu, bad, mine * kGroups + group);
+        const uint32_t i = base + mine * kGroups + group;
+        if (lane % kSame == 0 && i < n) score[i] = skip ? -kScoreLimit : ordered_score(s[0]);
+    }
+}
+
+// LANES = 0: one element at a time.
+template <typename T, int LANES, int VECS>
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p) {
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ SelectShared s;
@@ -331,7 +413,11 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
     for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) state[i] = need > 0 ? kOpen : kDropped;
     __syncthreads();
     if (need > 0) {
-        score_blocks<T>(p, p.tables + static_cast<size_t>(b) * p.pitch, head, weight, first, n, score);
+        const int32_t* table = p.tables + static_cast<size_t>(b) * p.pitch;
+        if constexpr (LANES == 0)
+            score_blocks<T>(p, table, head, weight, first, n, score);
+        else
+            score_blocks_vec<T, LANES, VECS>(p, table, head, weight, first, n, score);
         __syncthreads();
         take_best(score, state, n, first, need, s, cluster, rank);
     }
@@ -366,14 +452,29 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
     cluster_barrier(cluster);
 }
 
-template <typename T>
-int launch_select(const SelectParams& p, uint32_t segments, size_t smem, cudaStream_t st) {
+template <typename T, int LANES, int VECS>
+int launch_select_t(const SelectParams& p, uint32_t segments, size_t smem, cudaStream_t st) {
     static std::atomic<std::uint64_t> attr_done{0};
-    auto kern = select_kernel<T>;
+    auto kern = select_kernel<T, LANES, VECS>;
     const int rc = set_smem_limit_once(attr_done, reinterpret_cast<const void*>(kern), 200 * 1024,
                                        "cudaFuncSetAttribute(select_blocks)");
     if (rc != QVP_OK) return rc;
-    return launch_dependent("launch select_blocks", kern, dim3(segments * p.cluster), kSelThreads, smem, p.cluster, st, p);
+    return launch_dependent("launch select_blocks", kern, dim3(segments * p.cluster), kSelThreads, smem, p.cluster, st,
+                            p);
+}
+
+template <typename T>
+int launch_select(const SelectParams& p, uint32_t segments, size_t smem, cudaStream_t st) {
+    constexpr uint32_t V = 16 / sizeof(T);
+    const uint32_t vectors = 2 * p.D / V;
+    if (p.D % V != 0 || !aligned_to(p.summary, 16) || p.summary_stride % 16 != 0)
+        return launch_select_t<T, 0, 1>(p, segments, smem, st);
+    if (vectors <= 16) return launch_select_t<T, 16, 1>(p, segments, smem, st);
+    if (vectors <= 32) return launch_select_t<T, 32, 1>(p, segments, smem, st);
+    if constexpr (sizeof(T) == 4) {
+        if (vectors > 64) return launch_select_t<T, 32, 4>(p, segments, smem, st);
+    }
+    return launch_select_t<T, 32, 2>(p, segments, smem, st);
 }
 
 }  // namespace

@@ -69,7 +69,8 @@ struct TileShape {
     static constexpr uint32_t kRing = STAGES * kPiece;               // one warp's
     static constexpr uint32_t kBars = kTileWarps * kRing;            // offset of the barriers
     static constexpr uint32_t kStats = kBars + kTileWarps * STAGES * 8;  // m, l of 16 rows per warp, tokens seen
-    static constexpr uint32_t kSmem = kStats + kTileWarps * (32 * 4 + 16) + 1024;
+    static constexpr uint32_t kJoined = kStats + kTileWarps * (32 * 4 + 16);  // the same of the whole CTA
+    static constexpr uint32_t kSmem = kJoined + 32 * 4 + 16 + 1024;
     static_assert(kRing >= 16 * D * 4, "a warp's partial output takes the place of its ring");
 };
 
@@ -186,17 +187,17 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     const uint32_t b = seg / p.hkv, head = seg % p.hkv;
     const int G = static_cast<int>(min(p.group - blockIdx.y * 16, 16u));  // heads of this chunk
     const size_t h0 = static_cast<size_t>(head) * p.group + blockIdx.y * 16;
-    const int ctx = p.ctx[b];
-    if (ctx < 0 || static_cast<uint32_t>(ctx) > p.capacity) {  // the whole cluster
-        if (threadIdx.x == 0) record_error(p.err, kErrBadContext);
-        return;
-    }
     const int32_t* list = p.selected + static_cast<size_t>(seg) * p.keep;
     const int32_t* table = p.tables + static_cast<size_t>(b) * p.pitch;
     const uint32_t per_block = p.T / 16;
-    const uint32_t nblk = (static_cast<uint32_t>(ctx) + p.T - 1) / p.T;
     const uint64_t pieces = static_cast<uint64_t>(p.keep) * per_block;
     const uint32_t workers = cluster * kTileWarps, worker = rank * kTileWarps + warp;
+    // The lane's piece of a round of 32 per warp: its listed block (-1: none)
+    // and that block's frame. Neither load waits for the context length.
+    auto block_of = [&](uint64_t i) { return i < pieces ? list[i / per_block] : -1; };
+    auto frame_of = [&](int32_t blk) { return static_cast<uint32_t>(blk) < p.pitch ? table[blk] : -1; };
+    int32_t blk = block_of(worker + static_cast<uint64_t>(workers) * lane);
+    const int ctx = p.ctx[b];
 
     uint32_t qa[D / 16][4];
     {
@@ -213,6 +214,12 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             qa[ks][3] = g + 8 < G ? q_hi[k0 + 4] : 0u;
         }
     }
+    int32_t frame = frame_of(blk);
+    if (ctx < 0 || static_cast<uint32_t>(ctx) > p.capacity) {  // the whole cluster
+        if (threadIdx.x == 0) record_error(p.err, kErrBadContext);
+        return;
+    }
+    const uint32_t nblk = (static_cast<uint32_t>(ctx) + p.T - 1) / p.T;
     WarpState<D> st;
     st.reset();
     uint32_t seen = 0;                      // tokens attended by this warp
@@ -220,28 +227,22 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     bool alive = true;
     const uint64_t policy = l2_policy_evict_first();
 
-    // Lane l looks up the warp's l-th next piece: its K row in the pool and
-    // the tokens it has below the context (0: nothing to attend).
     for (uint64_t base = worker; alive && base < pieces; base += static_cast<uint64_t>(workers) * 32) {
+        // the piece's K row in the pool and the tokens it has below the
+        // context (0: nothing to attend)
         const uint64_t i = base + static_cast<uint64_t>(workers) * lane;
+        const uint32_t first = static_cast<uint32_t>(i % per_block) * 16;
         int valid = 0, krow = 0;
-        if (i < pieces && ctx > 0) {
-            const int32_t blk = list[i / per_block];
-            const uint32_t first = static_cast<uint32_t>(i % per_block) * 16;
-            if (blk >= 0) {
-                if (static_cast<uint32_t>(blk) >= nblk) {
-                    record_error(p.err, kErrBadBlockId);
-                } else {
-                    const int32_t id = table[blk];
-                    if (static_cast<uint32_t>(id) >= p.num_blocks)
-                        record_error(p.err, kErrBadBlockId);
-                    else {
-                        valid = max(0, min(16, ctx - static_cast<int>(static_cast<uint32_t>(blk) * p.T + first)));
-                        krow = static_cast<int>(((static_cast<uint32_t>(id) * p.num_layers + p.layer) * 2) * p.T + first);
-                    }
-                }
+        if (blk >= 0 && ctx > 0) {
+            if (static_cast<uint32_t>(blk) >= nblk || static_cast<uint32_t>(frame) >= p.num_blocks) {
+                record_error(p.err, kErrBadBlockId);
+            } else {
+                valid = max(0, min(16, ctx - static_cast<int>(static_cast<uint32_t>(blk) * p.T + first)));
+                krow = static_cast<int>(((static_cast<uint32_t>(frame) * p.num_layers + p.layer) * 2) * p.T + first);
             }
         }
+        blk = block_of(i + static_cast<uint64_t>(workers) * 32);  // of the next round
+        frame = frame_of(blk);
         uint32_t to_issue = __ballot_sync(0xffffffffu, valid > 0), to_use = to_issue;
         auto issue = [&]() {
             const int from = __ffs(to_issue) - 1;
@@ -311,43 +312,82 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         }
         if (lane == 0) reinterpret_cast<uint32_t*>(stat)[32] = seen;
     }
-    auto barrier = [&]() {
-        if (cluster > 1)
-            cg::this_cluster().sync();
-        else
-            __syncthreads();
-    };
-    barrier();
-    // Each CTA of the cluster writes its share of the output, two elements a thread.
+    __syncthreads();
+    // Join the warps, two elements a thread: straight to the output, or to the
+    // first warp's place for the cluster.
+    const float* stats = reinterpret_cast<const float*>(smem + S::kStats);
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + (static_cast<size_t>(b) * p.hq + h0) * D;
-    for (uint32_t i = rank * kTileThreads + threadIdx.x; i < static_cast<uint32_t>(G) * (D / 2);
-         i += cluster * kTileThreads) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int w = 0; w < kTileWarps; ++w) any |= reinterpret_cast<const uint32_t*>(stats)[w * 36 + 32];
+    auto write_out = [&](uint32_t g, uint32_t d, float x, float y, float sum) {
+        const float inv = 1.f / sum;
+        *reinterpret_cast<uint32_t*>(out + g * D + d) = any != 0 ? pack_bf16x2(x * inv, y * inv) : 0u;
+    };
+    // without a score above -inf a partial's sums are 0, or NaN from a NaN score
+    auto weight_of = [](float m, float M) { return m == -INFINITY ? 1.f : exp2f(m - M); };
+    for (uint32_t i = threadIdx.x; i < static_cast<uint32_t>(G) * (D / 2); i += kTileThreads) {
         const uint32_t g = i / (D / 2), d = i % (D / 2) * 2;
         float M = -INFINITY;
-        uint32_t any = 0;
-        for (uint32_t w = 0; w < workers; ++w) {
-            const uint8_t* at = cluster > 1 ? cg::this_cluster().map_shared_rank(smem, w / kTileWarps) : smem;
-            const float* stat = reinterpret_cast<const float*>(at + S::kStats) + (w % kTileWarps) * 36;
-            M = fmaxf(M, stat[g]);
-            any |= reinterpret_cast<const uint32_t*>(stat)[32];
-        }
+#pragma unroll
+        for (int w = 0; w < kTileWarps; ++w) M = fmaxf(M, stats[w * 36 + g]);
         float sum = 0.f, x = 0.f, y = 0.f;
-        for (uint32_t w = 0; w < workers; ++w) {
-            const uint8_t* at = cluster > 1 ? cg::this_cluster().map_shared_rank(smem, w / kTileWarps) : smem;
-            const float* stat = reinterpret_cast<const float*>(at + S::kStats) + (w % kTileWarps) * 36;
-            const float2 o = *reinterpret_cast<const float2*>(at + (w % kTileWarps) * S::kRing + (g * D + d) * 4);
-            const float m = stat[g];
-            // without a score above -inf the sums are 0, or NaN from a NaN score
-            const float weight = m == -INFINITY ? 1.f : exp2f(m - M);
-            sum += weight * stat[16 + g];
+#pragma unroll
+        for (int w = 0; w < kTileWarps; ++w) {
+            const float2 o = *reinterpret_cast<const float2*>(smem + w * S::kRing + (g * D + d) * 4);
+            const float weight = weight_of(stats[w * 36 + g], M);
+            sum += weight * stats[w * 36 + 16 + g];
             x += weight * o.x;
             y += weight * o.y;
         }
-        const float inv = any != 0 ? 1.f / sum : 0.f;
-        *reinterpret_cast<uint32_t*>(out + g * D + d) = any != 0 ? pack_bf16x2(x * inv, y * inv) : 0u;
+        if (cluster == 1) {
+            write_out(g, d, x, y, sum);
+        } else {
+            *reinterpret_cast<float2*>(smem + (g * D + d) * 4) = make_float2(x, y);
+            if (d == 0) {
+                float* joined = reinterpret_cast<float*>(smem + S::kJoined);
+                joined[g] = M;
+                joined[16 + g] = sum;
+                if (g == 0) reinterpret_cast<uint32_t*>(joined)[32] = any;
+            }
+        }
+    }
+    if (cluster == 1) return;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    for (uint32_t i = rank * kTileThreads + threadIdx.x; i < static_cast<uint32_t>(G) * (D / 2);
+         i += cluster * kTileThreads) {
+        const uint32_t g = i / (D / 2), d = i % (D / 2) * 2;
+        float m[kTileMaxCluster], l[kTileMaxCluster];
+        float2 o[kTileMaxCluster];
+        float M = -INFINITY;
+#pragma unroll
+        for (uint32_t r = 0; r < kTileMaxCluster; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+            o[r] = make_float2(0.f, 0.f);
+            if (r < cluster) {
+                const uint8_t* at = cl.map_shared_rank(smem, r);
+                const float* joined = reinterpret_cast<const float*>(at + S::kJoined);
+                m[r] = joined[g];
+                l[r] = joined[16 + g];
+                any |= reinterpret_cast<const uint32_t*>(joined)[32];
+                o[r] = *reinterpret_cast<const float2*>(at + (g * D + d) * 4);
+            }
+            M = fmaxf(M, m[r]);
+        }
+        float sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+        for (uint32_t r = 0; r < kTileMaxCluster; ++r) {
+            const float weight = weight_of(m[r], M);
+            sum += weight * l[r];
+            x += weight * o[r].x;
+            y += weight * o[r].y;
+        }
+        write_out(g, d, x, y, sum);
     }
     // no CTA leaves while another may read its shared memory
-    barrier();
+    cl.sync();
 }
 
 template <int D, int STAGES, bool PAIR, bool SPLIT>
@@ -705,9 +745,9 @@ extern "C" int qvp_decode_selected(const qvp_decode_selected_args* args, qvp_str
     if (tile) {
         const uint64_t pieces = static_cast<uint64_t>(p.keep) * (p.T / 16);
         p.cluster = 1;
-        while (p.cluster < kTileMaxCluster && segments * p.cluster < 2 * sms && pieces > 2 * kTileWarps * p.cluster)
+        // two CTAs are resident per SM: split a list while the whole grid still is
+        while (p.cluster < kTileMaxCluster && segments * p.cluster * 2 <= 2 * sms && pieces > kTileWarps * p.cluster)
             p.cluster *= 2;
-        if (segments * p.cluster > 0x7fffffffu) return fail(QVP_ERR_UNSUPPORTED, "more than 2^31 sequences and heads");
         return p.D == 128 ? launch_tile<128, 3>(p, a, static_cast<uint32_t>(segments), st)
                           : launch_tile<64, 6>(p, a, static_cast<uint32_t>(segments), st);
     }
