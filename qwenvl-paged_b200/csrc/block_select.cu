@@ -6,10 +6,13 @@
 //
 // The score of a group is one product of length 2 * head_dim with the block's
 // summary row, so summaries are read once for all heads of the group and HBM
-// bounds the call. Sums are 64-bit: a product of two bf16 has 16 significant
-// bits and their sum rarely needs more than 53, so the choice between blocks
-// of nearly the same score does not depend on the order of the sum (32-bit
-// sums in another order swap about one border block in a hundred rows).
+// bounds the call. The choice is made by 64-bit sums: a product of two bf16
+// has 16 significant bits and their sum rarely needs more than 53, so it does
+// not depend on the order of the sum (32-bit sums in another order swap about
+// one border block in a hundred rows). For bf16 only the blocks near the
+// border are summed that way: the tensor cores score all of them first, with
+// a bound on their error, and what lies within it of the border is scored
+// again.
 //
 // A cluster of CTAs serves one (sequence, kv head): each scores its part of
 // the blocks into shared memory, and they agree on the border of the best
@@ -33,7 +36,7 @@ constexpr int kSelWarps = kSelThreads / 32;
 constexpr uint32_t kSelBins = 512;
 constexpr uint32_t kSelBorder = kSelThreads;      // border members ranked in one go, one per thread
 constexpr uint32_t kSelMaxCluster = 8;
-constexpr uint32_t kSelMaxChunk = 20480;          // blocks one CTA can hold (8-byte score, 1-byte state)
+constexpr uint32_t kSelMaxChunk = 14336;          // blocks one CTA can hold: 13 bytes each of 200 KiB
 
 // States of a block during the search.
 enum : uint8_t { kOpen = 0, kTaken = 1, kDropped = 2 };
@@ -61,15 +64,18 @@ struct SelectShared {
     uint32_t total[kSelBins];         // the cluster's
     double border_score[kSelBorder];  // this CTA's open blocks, when they are few
     uint32_t border_block[kSelBorder];
-    double all_score[kSelBorder];     // the cluster's
+    double all_score[kSelBorder];     // the cluster's, by rank
     uint32_t all_block[kSelBorder];
     double lo, hi;                    // range of this CTA's open scores
     double warp_lo[kSelWarps], warp_hi[kSelWarps];
+    float key_lo, key_hi, top;        // the same of the keys; largest sum of a score's terms without their signs
+    float warp_key_lo[kSelWarps], warp_key_hi[kSelWarps], warp_top[kSelWarps];
     uint32_t warp_sum[kSelWarps];
     uint32_t border_count;
     uint32_t open_count;              // this CTA's open blocks
-    uint32_t taken;                   // this CTA's taken blocks
-    uint32_t bin, above;              // the border's bin, open scores in higher bins
+    uint32_t taken;                   // this CTA's blocks that are taken for sure
+    uint32_t before;                  // border blocks taken by lower ranks
+    uint32_t bin;                     // the border's bin
 };
 
 // Infinities become bounds that no finite score reaches (products of two
@@ -81,11 +87,26 @@ __device__ __forceinline__ double ordered_score(double s) {
     return fmax(s, -kScoreLimit) + 0.0;  // -0 becomes +0
 }
 
-// Bin of s in [lo, hi], never decreasing in s; lo falls in bin 0 and hi in
-// the last one.
+// A score in 32 bits: never decreasing in it, and any two of them a finite
+// distance apart. NaN counts as +infinity.
+constexpr float kKeyLimit = 8e37f;
+__device__ __forceinline__ float ordered_key(float s) {
+    if (!(s < kKeyLimit)) return kKeyLimit;
+    return fmaxf(s, -kKeyLimit);
+}
+__device__ __forceinline__ float score_key(double s) { return ordered_key(static_cast<float>(s)); }
+
+// Bin of a score or key, never decreasing in it; lo and below fall in bin 0,
+// hi and above in the last one.
 __device__ __forceinline__ uint32_t score_bin(double s, double lo, double per_bin) {
     const double x = (s - lo) * per_bin;
-    return x >= static_cast<double>(kSelBins - 1) ? kSelBins - 1 : static_cast<uint32_t>(x);
+    if (x >= static_cast<double>(kSelBins - 1)) return kSelBins - 1;
+    return x > 0.0 ? static_cast<uint32_t>(x) : 0u;
+}
+__device__ __forceinline__ uint32_t key_bin(float k, float lo, float per_bin) {
+    const float x = (k - lo) * per_bin;  // NaN (0 * inf) only for k = lo
+    if (x >= static_cast<float>(kSelBins - 1)) return kSelBins - 1;
+    return x > 0.f ? static_cast<uint32_t>(x) : 0u;
 }
 
 __device__ __forceinline__ void cluster_barrier(uint32_t cluster) {
@@ -106,199 +127,460 @@ __device__ __forceinline__ double warp_sum(double x) {
     return x;
 }
 
-// Number of set flags over the CTA; every thread gets it. Ends with a barrier.
-__device__ __forceinline__ uint32_t cta_count(uint32_t mine, SelectShared& s) {
-    const uint32_t w = __reduce_add_sync(0xffffffffu, mine);
-    if ((threadIdx.x & 31) == 0) s.warp_sum[threadIdx.x >> 5] = w;
-    __syncthreads();
-    uint32_t n = 0;
+// Exclusive position of this thread's `mine` among the CTA's, in thread order;
+// `all` gets the total. One barrier.
+__device__ __forceinline__ uint32_t cta_scan(uint32_t mine, uint32_t& all, SelectShared& s) {
+    uint32_t upto = mine;
 #pragma unroll
-    for (int i = 0; i < kSelWarps; ++i) n += s.warp_sum[i];
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        if ((threadIdx.x & 31) >= static_cast<uint32_t>(o)) upto += x;
+    }
+    if ((threadIdx.x & 31) == 31) s.warp_sum[threadIdx.x >> 5] = upto;
     __syncthreads();
-    return n;
+    uint32_t before = upto - mine;
+    all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kSelWarps; ++w) {
+        if (w < (threadIdx.x >> 5)) before += s.warp_sum[w];
+        all += s.warp_sum[w];
+    }
+    return before;
 }
 
-// Range of this CTA's open scores into s.lo, s.hi.
-__device__ __forceinline__ void open_range(const double* score, const uint8_t* state, uint32_t n, SelectShared& s) {
-    double lo = INFINITY, hi = -INFINITY;
-    for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) {
-        if (state[i] == kOpen) {
-            lo = fmin(lo, score[i]);
-            hi = fmax(hi, score[i]);
-        }
+// The score of one block, any head_dim and alignment: lanes along the row.
+template <typename T>
+__device__ __forceinline__ double score_block(const SelectParams& p, int32_t id, uint32_t head, const double* weight) {
+    const T* row = reinterpret_cast<const T*>(p.summary + static_cast<size_t>(id) * p.summary_stride) +
+                   (static_cast<size_t>(p.layer) * p.hkv + head) * 2 * p.D;
+    double s = 0.0;
+#pragma unroll 8
+    for (uint32_t e = threadIdx.x & 31; e < 2 * p.D; e += 32)
+        s += static_cast<double>(to_float<T>(row[e])) * weight[e];
+    return ordered_score(warp_sum(s));
+}
+
+// The scores of K blocks, their rows in flight together; ids outside the pool
+// score lowest.
+template <typename T, int K>
+__device__ __forceinline__ void score_several(const SelectParams& p, const int32_t (&ids)[K], uint32_t head,
+                                              const double* weight, double (&s)[K]) {
+    const T* row[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        row[k] = reinterpret_cast<const T*>(
+                     p.summary + static_cast<size_t>(static_cast<uint32_t>(ids[k]) < p.num_blocks ? ids[k] : 0) *
+                                     p.summary_stride) +
+                 (static_cast<size_t>(p.layer) * p.hkv + head) * 2 * p.D;
+        s[k] = 0.0;
     }
+#pragma unroll 4
+    for (uint32_t e = threadIdx.x & 31; e < 2 * p.D; e += 32) {
+        const double w = weight[e];
+#pragma unroll
+        for (int k = 0; k < K; ++k) s[k] += static_cast<double>(to_float<T>(row[k][e])) * w;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        s[k] = ordered_score(warp_sum(s[k]));
+        if (static_cast<uint32_t>(ids[k]) >= p.num_blocks) s[k] = -kScoreLimit;
+    }
+}
+
+// What a CTA works on: its part of the blocks of one (sequence, kv head).
+struct SelectPart {
+    const int32_t* table;   // ids of its blocks
+    const double* weight;   // [down D | up D], against a summary's [min D | max D]
+    float* key;             // scores in 32 bits
+    double* score;          // exact scores: of all blocks, or, after approximate ones, of those left open
+    uint8_t* state;
+    uint32_t first, n;      // its blocks
+    uint32_t head, rank;
+};
+
+// `mine` of every CTA of the cluster: lane r gets that of rank r, lanes past
+// the cluster `none`.
+template <typename V>
+__device__ __forceinline__ V of_every_rank(V* mine, uint32_t cluster, V none) {
+    const uint32_t lane = threadIdx.x & 31;
+    return lane < cluster ? *of_rank(mine, cluster, lane) : none;
+}
+
+// The bin in which, counted from the top, the `left`-th score lies. One warp.
+__device__ __forceinline__ void find_border(const uint32_t* total, uint32_t left, SelectShared& s) {
+    const uint32_t lane = threadIdx.x & 31;
+    // lane l holds the bins of the l-th slice from the top
+    constexpr uint32_t kPer = kSelBins / 32;
+    const uint32_t above_mine = kSelBins - lane * kPer;  // bins [above_mine - kPer, above_mine)
+    uint32_t count[kPer], mine = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) mine += count[i] = total[above_mine - 1 - i];
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= static_cast<uint32_t>(o)) upto += x;
+    }
+    uint32_t above = upto - mine;
+    if (above < left && left <= upto) {
+        uint32_t bin = above_mine;
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; ++i) {
+            if (above < left) {
+                above += count[i];
+                --bin;
+            }
+        }
+        s.bin = bin;
+    }
+}
+
+// Takes the `need` best of the cluster's blocks (there are more), by value
+// and, on a tie, the lower block; blocks of a lower rank are lower. key_lo and
+// key_hi: the range of this thread's keys. The keys are part.score in 32 bits
+// where error_scale is 0, else scores that are off by less than error_scale
+// times the largest `top` of a thread, and part.score is not yet there. Marks
+// this CTA's blocks in part.state and returns how many the lower ranks took.
+// After it no CTA reads another's shared memory; a cluster has arrived at its
+// barrier once.
+//
+// The first cut is by keys. Where it leaves more than kSelBorder blocks, 64-bit
+// cuts follow.
+template <typename T>
+__device__ uint32_t take_best(const SelectParams& p, const SelectPart& part, uint32_t need, float key_lo, float key_hi,
+                              float top, double error_scale, SelectShared& s) {
+    const uint32_t cluster = p.cluster, rank = part.rank, n = part.n;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double* const score = part.score;
+    uint8_t* const state = part.state;
+    uint32_t left = need;   // to take among the open blocks
+
+    // the range of the keys
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        lo = fmin(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmax(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        key_lo = fminf(key_lo, __shfl_xor_sync(0xffffffffu, key_lo, o));
+        key_hi = fmaxf(key_hi, __shfl_xor_sync(0xffffffffu, key_hi, o));
+        top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
-    if ((threadIdx.x & 31) == 0) {
-        s.warp_lo[threadIdx.x >> 5] = lo;
-        s.warp_hi[threadIdx.x >> 5] = hi;
+    if (lane == 0) {
+        s.warp_key_lo[warp] = key_lo;
+        s.warp_key_hi[warp] = key_hi;
+        s.warp_top[warp] = top;
     }
+    for (uint32_t i = threadIdx.x; i < kSelBins; i += kSelThreads) s.hist[i] = 0;
+    if (threadIdx.x == 0) s.taken = s.border_count = s.before = 0;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < kSelWarps; ++i) {
-            lo = fmin(lo, s.warp_lo[i]);
-            hi = fmax(hi, s.warp_hi[i]);
-        }
-        s.lo = lo;
-        s.hi = hi;
-    }
-}
-
-// Takes the `need` best of the cluster's open blocks (there are more), given
-// by value and, on a tie, the lower block. Blocks of a lower rank are lower.
-__device__ void take_best(const double* score, uint8_t* state, uint32_t n, uint32_t first, uint32_t need,
-                          SelectShared& s, uint32_t cluster, uint32_t rank) {
-    for (;;) {
-        open_range(score, state, n, s);
-        for (uint32_t i = threadIdx.x; i < kSelBins; i += kSelThreads) s.hist[i] = 0;
-        cluster_barrier(cluster);
-        double lo = INFINITY, hi = -INFINITY;
-        for (uint32_t r = 0; r < cluster; ++r) {
-            lo = fmin(lo, *of_rank(&s.lo, cluster, r));
-            hi = fmax(hi, *of_rank(&s.hi, cluster, r));
-        }
-        if (!(lo < hi)) break;  // all open scores are the same
-        const double per_bin = static_cast<double>(kSelBins) / (hi - lo);
-        for (uint32_t i = threadIdx.x; i < n; i += kSelThreads)
-            if (state[i] == kOpen) atomicAdd(&s.hist[score_bin(score[i], lo, per_bin)], 1u);
-        cluster_barrier(cluster);
-        for (uint32_t i = threadIdx.x; i < kSelBins; i += kSelThreads) {
-            uint32_t t = 0;
-            for (uint32_t r = 0; r < cluster; ++r) t += *of_rank(&s.hist[i], cluster, r);
-            s.total[i] = t;
-        }
-        if (threadIdx.x == 0) s.border_count = 0;
-        __syncthreads();
-        if (threadIdx.x < 32) {
-            // lane l holds the bins of the l-th slice from the top
-            constexpr uint32_t kPer = kSelBins / 32;
-            const uint32_t top = kSelBins - threadIdx.x * kPer;  // bins [top - kPer, top)
-            uint32_t mine = 0;
-            for (uint32_t i = 0; i < kPer; ++i) mine += s.total[top - 1 - i];
-            uint32_t upto = mine;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
-                if (threadIdx.x >= static_cast<uint32_t>(o)) upto += x;
+    for (int i = 0; i < kSelWarps; ++i) {
+        key_lo = fminf(key_lo, s.warp_key_lo[i]);
+        key_hi = fmaxf(key_hi, s.warp_key_hi[i]);
+        top = max_nan(top, s.warp_top[i]);
+    }
+    if (cluster > 1) {
+        if (threadIdx.x == 0) {
+            s.key_lo = key_lo;
+            s.key_hi = key_hi;
+            s.top = top;
+        }
+        cg::this_cluster().sync();
+        key_lo = of_every_rank(&s.key_lo, cluster, key_lo);
+        key_hi = of_every_rank(&s.key_hi, cluster, key_hi);
+        top = of_every_rank(&s.top, cluster, top);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {  // at most 8 ranks
+            key_lo = fminf(key_lo, __shfl_xor_sync(0xffffffffu, key_lo, o));
+            key_hi = fmaxf(key_hi, __shfl_xor_sync(0xffffffffu, key_hi, o));
+            top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        }
+        key_lo = __shfl_sync(0xffffffffu, key_lo, 0);
+        key_hi = __shfl_sync(0xffffffffu, key_hi, 0);
+        top = __shfl_sync(0xffffffffu, top, 0);
+    }
+    // Scores further apart than `slack` are in their true order: twice the
+    // error, 1e-30 for products below the normal range, and the rounding of
+    // key - slack. Beyond 1e30 (or NaN) the 32-bit scores may have overflowed:
+    // there is no bound, and every block is scored again.
+    const bool approximate = error_scale > 0.0;
+    const float slack = approximate ? static_cast<float>(2.0 * error_scale * static_cast<double>(top)) * 1.0001f +
+                                          1e-30f + 0x1p-22f * fmaxf(fabsf(key_lo), fabsf(key_hi))
+                                    : 0.f;
+    const bool unbounded = !(slack < 1e30f);
+    const float per_key = static_cast<float>(kSelBins) / (key_hi - key_lo);
+    bool cut_by_key = true;
+    double lo = 0.0, hi = 0.0;
+
+    for (;;) {
+        double per_bin = 0.0;
+        if (!cut_by_key) {
+            // the range of the open scores
+            lo = INFINITY;
+            hi = -INFINITY;
+            for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) {
+                if (state[i] == kOpen) {
+                    lo = fmin(lo, score[i]);
+                    hi = fmax(hi, score[i]);
+                }
             }
-            uint32_t above = upto - mine;
-            if (above < need && need <= upto) {
-                uint32_t bin = top - 1;
-                while (above + s.total[bin] < need) above += s.total[bin--];
-                s.bin = bin;
-                s.above = above;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                lo = fmin(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = fmax(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            }
+            if (lane == 0) {
+                s.warp_lo[warp] = lo;
+                s.warp_hi[warp] = hi;
+            }
+            for (uint32_t i = threadIdx.x; i < kSelBins; i += kSelThreads) s.hist[i] = 0;
+            if (threadIdx.x == 0) s.border_count = s.before = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kSelWarps; ++i) {
+                lo = fmin(lo, s.warp_lo[i]);
+                hi = fmax(hi, s.warp_hi[i]);
+            }
+            if (cluster > 1) {
+                if (threadIdx.x == 0) {
+                    s.lo = lo;
+                    s.hi = hi;
+                }
+                cg::this_cluster().sync();
+                for (uint32_t r = 0; r < cluster; ++r) {
+                    lo = fmin(lo, *of_rank(&s.lo, cluster, r));
+                    hi = fmax(hi, *of_rank(&s.hi, cluster, r));
+                }
+            }
+            if (!(lo < hi)) break;  // all open scores are the same
+            per_bin = static_cast<double>(kSelBins) / (hi - lo);
+        }
+        if (cut_by_key) {
+#pragma unroll 4
+            for (uint32_t i = threadIdx.x; i < n; i += kSelThreads)
+                atomicAdd(&s.hist[key_bin(part.key[i], key_lo, per_key)], 1u);
+        } else {
+            for (uint32_t i = threadIdx.x; i < n; i += kSelThreads)
+                if (state[i] == kOpen) atomicAdd(&s.hist[score_bin(score[i], lo, per_bin)], 1u);
+        }
+        cluster_barrier(cluster);
+        if (cluster > 1) {
+            for (uint32_t i = threadIdx.x; i < kSelBins; i += kSelThreads) {
+                uint32_t count = 0;
+#pragma unroll
+                for (uint32_t r = 0; r < kSelMaxCluster; ++r)
+                    if (r < cluster) count += *of_rank(&s.hist[i], cluster, r);
+                s.total[i] = count;
+            }
+            __syncthreads();
+        }
+        if (warp == 0) find_border(cluster > 1 ? s.total : s.hist, left, s);
+        __syncthreads();
+        const uint32_t bin = s.bin;
+        uint32_t taken = 0;
+        auto list_open = [&](uint32_t i) {
+            const uint32_t at = atomicAdd(&s.border_count, 1u);
+            if (at < kSelBorder) {
+                s.border_block[at] = part.first + i;
+                if (!cut_by_key || !approximate) s.border_score[at] = score[i];
+            }
+        };
+        if (cut_by_key) {
+#pragma unroll 4
+            for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) {
+                const float k = part.key[i];
+                const bool above = key_bin(k - slack, key_lo, per_key) > bin && !unbounded;
+                const bool below = key_bin(k + slack, key_lo, per_key) < bin && !unbounded;
+                state[i] = above ? kTaken : below ? kDropped : kOpen;
+                taken += above;
+                if (!above && !below) list_open(i);
+            }
+        } else {
+            for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) {
+                if (state[i] != kOpen) continue;
+                const uint32_t x = score_bin(score[i], lo, per_bin);
+                if (x != bin) state[i] = x > bin ? kTaken : kDropped;
+                taken += x > bin;
+                if (x == bin) list_open(i);
+            }
+        }
+        taken = __reduce_add_sync(0xffffffffu, taken);
+        if (lane == 0 && taken > 0) atomicAdd(&s.taken, taken);
+        if (cut_by_key && approximate) {
+            __syncthreads();
+            // in 64 bits now: from the list, or, where it overflowed, from all
+            const bool listed = s.border_count <= kSelBorder;
+            const uint32_t count = listed ? s.border_count : n;
+            constexpr int K = 2;
+            for (uint32_t k0 = warp * K; k0 < count; k0 += kSelWarps * K) {
+                uint32_t at[K];
+                int32_t ids[K];
+                double x[K];
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const uint32_t i = min(k0 + k, count - 1);
+                    at[k] = listed ? s.border_block[i] - part.first : i;
+                    ids[k] = part.table[at[k]];
+                }
+                score_several<T, K>(p, ids, part.head, part.weight, x);
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if (lane == 0 && k0 + k < count && state[at[k]] == kOpen) {
+                        score[at[k]] = x[k];
+                        if (listed) s.border_score[k0 + k] = x[k];
+                    }
+                }
+            }
+        }
+        cut_by_key = false;
+        cluster_barrier(cluster);  // the bins have been read, the border lists and counts are there
+        // members and taken blocks of the ranks up to and with this lane's
+        const uint32_t my_count = of_every_rank(&s.border_count, cluster, 0u);
+        uint32_t members_upto = my_count, taken_upto = of_every_rank(&s.taken, cluster, 0u);
+#pragma unroll
+        for (int o = 1; o < static_cast<int>(kSelMaxCluster); o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, members_upto, o);
+            const uint32_t y = __shfl_up_sync(0xffffffffu, taken_upto, o);
+            if (lane >= static_cast<uint32_t>(o)) {
+                members_upto += x;
+                taken_upto += y;
+            }
+        }
+        const uint32_t members = __shfl_sync(0xffffffffu, members_upto, cluster - 1);
+        left = need - __shfl_sync(0xffffffffu, taken_upto, cluster - 1);
+        if (members > kSelBorder) {
+            cluster_barrier(cluster);  // the counts have been read
+            continue;
+        }
+        const uint32_t mine_from = __shfl_sync(0xffffffffu, members_upto - my_count, rank);
+        const uint32_t taken_before = rank > 0 ? __shfl_sync(0xffffffffu, taken_upto, rank - 1) : 0u;
+        const double* scores = s.border_score;
+        const uint32_t* blocks = s.border_block;
+        if (cluster > 1) {
+            uint32_t from = 0, owner = 0;
+#pragma unroll
+            for (uint32_t r = 0; r + 1 < kSelMaxCluster; ++r) {
+                const uint32_t end = __shfl_sync(0xffffffffu, members_upto, r);
+                if (r + 1 < cluster && threadIdx.x >= end) {
+                    from = end;
+                    owner = r + 1;
+                }
+            }
+            if (threadIdx.x < members) {
+                s.all_score[threadIdx.x] = of_rank(s.border_score, cluster, owner)[threadIdx.x - from];
+                s.all_block[threadIdx.x] = of_rank(s.border_block, cluster, owner)[threadIdx.x - from];
+            }
+            scores = s.all_score;
+            blocks = s.all_block;
+            __syncthreads();
+            cg::this_cluster().barrier_arrive();
+        }
+        // Rank the border's members, one per thread, those of every CTA.
+        if (threadIdx.x < members) {
+            const double mine = scores[threadIdx.x];
+            const uint32_t block = blocks[threadIdx.x];
+            uint32_t better = 0;
+#pragma unroll 4
+            for (uint32_t i = 0; i < members; ++i)
+                better += scores[i] > mine || (scores[i] == mine && blocks[i] < block);
+            if (threadIdx.x < mine_from) {
+                if (better < left) atomicAdd(&s.before, 1u);
+            } else if (threadIdx.x - mine_from < s.border_count) {
+                state[block - part.first] = better < left ? kTaken : kDropped;
             }
         }
         __syncthreads();
-        const uint32_t bin = s.bin, members = s.total[s.bin];
-        need -= s.above;
-        const bool whole = members == need, few = members <= kSelBorder;
-        for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) {
-            if (state[i] != kOpen) continue;
-            const uint32_t x = score_bin(score[i], lo, per_bin);
-            if (x > bin || (x == bin && whole)) {
-                state[i] = kTaken;
-            } else if (x < bin) {
-                state[i] = kDropped;
-            } else if (few) {
-                const uint32_t at = atomicAdd(&s.border_count, 1u);
-                s.border_score[at] = score[i];
-                s.border_block[at] = first + i;
-            }
-        }
-        if (whole) {
-            __syncthreads();
-            return;
-        }
-        if (few) {
-            cluster_barrier(cluster);
-            uint32_t from = 0;
-            for (uint32_t r = 0; r < cluster; ++r) {
-                const uint32_t c = *of_rank(&s.border_count, cluster, r);
-                for (uint32_t i = threadIdx.x; i < c; i += kSelThreads) {
-                    s.all_score[from + i] = of_rank(s.border_score, cluster, r)[i];
-                    s.all_block[from + i] = of_rank(s.border_block, cluster, r)[i];
-                }
-                from += c;
-            }
-            __syncthreads();
-            if (threadIdx.x < s.border_count) {
-                const double mine = s.border_score[threadIdx.x];
-                const uint32_t block = s.border_block[threadIdx.x];
-                uint32_t better = 0;
-                for (uint32_t i = 0; i < members; ++i)
-                    better += s.all_score[i] > mine || (s.all_score[i] == mine && s.all_block[i] < block);
-                state[block - first] = better < need ? kTaken : kDropped;
-            }
-            __syncthreads();
-            return;
-        }
-        cluster_barrier(cluster);  // the others have read this CTA's bins
+        return taken_before + s.before;
     }
     // Equal scores: the lowest blocks, so the lower ranks first.
     uint32_t mine = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) mine += state[i] == kOpen;
-    const uint32_t open = cta_count(mine, s);
+    const uint32_t per = (n + kSelThreads - 1) / kSelThreads;  // in block order: a run of blocks per thread
+    const uint32_t run = min(threadIdx.x * per, n), end = min(run + per, n);
+    for (uint32_t i = run; i < end; ++i) mine += state[i] == kOpen;
+    uint32_t open;
+    uint32_t ahead = cta_scan(mine, open, s);
     if (threadIdx.x == 0) s.open_count = open;
     cluster_barrier(cluster);
-    uint32_t before = 0;
-    for (uint32_t r = 0; r < rank; ++r) before += *of_rank(&s.open_count, cluster, r);
-    uint32_t left = need > before ? need - before : 0;
-    for (uint32_t i0 = 0; i0 < n; i0 += kSelThreads) {  // in block order
-        const uint32_t i = i0 + threadIdx.x;
-        const bool is = i < n && state[i] == kOpen;
-        const uint32_t votes = __ballot_sync(0xffffffffu, is);
-        if ((threadIdx.x & 31) == 0) s.warp_sum[threadIdx.x >> 5] = __popc(votes);
+    uint32_t at = 0;
+    for (uint32_t r = 0; r < rank; ++r) {
+        const uint32_t c = min(*of_rank(&s.open_count, cluster, r), left);
+        at += c + *of_rank(&s.taken, cluster, r);
+        left -= c;
+    }
+    if (cluster > 1) {
         __syncthreads();
-        uint32_t at = __popc(votes & ((1u << (threadIdx.x & 31)) - 1u)), all = 0;
-        for (uint32_t w = 0; w < kSelWarps; ++w) {
-            if (w < (threadIdx.x >> 5)) at += s.warp_sum[w];
-            all += s.warp_sum[w];
+        cg::this_cluster().barrier_arrive();
+    }
+    for (uint32_t i = run; i < end; ++i)
+        if (state[i] == kOpen) state[i] = ahead++ < left ? kTaken : kDropped;
+    __syncthreads();
+    return at;
+}
+
+// Sums over the query heads of the group: [down D | up D].
+template <typename T>
+__device__ __forceinline__ void make_weights(const SelectParams& p, uint32_t b, uint32_t head, double* weight) {
+    for (uint32_t d = threadIdx.x; d < p.D; d += kSelThreads) {
+        const T* q = static_cast<const T*>(p.q) + b * p.q_pitch + static_cast<size_t>(head) * p.group * p.D + d;
+        double up = 0.0, down = 0.0;
+#pragma unroll 8
+        for (uint32_t g = 0; g < p.group; ++g) {
+            const double x = static_cast<double>(to_float<T>(q[static_cast<size_t>(g) * p.D]));
+            // a NaN goes to both sums
+            if (!(x < 0.0)) up += x;
+            if (!(x > 0.0)) down += x;
         }
-        if (is) state[i] = at < left ? kTaken : kDropped;
-        left = left > all ? left - all : 0;
-        __syncthreads();
+        weight[d] = down;
+        weight[p.D + d] = up;
     }
 }
 
-// Scores of blocks [first, first + n) of one (sequence, kv head), any head_dim
-// and alignment: a warp per block, lanes along the row.
-template <typename T>
-__device__ __forceinline__ void score_blocks(const SelectParams& p, const int32_t* table, uint32_t head,
-                                             const double* weight, uint32_t first, uint32_t n, double* score) {
-    const uint32_t lane = threadIdx.x & 31;
-    for (uint32_t i = threadIdx.x >> 5; i < n; i += kSelWarps) {
-        const int32_t id = table[first + i];
-        double s = -kScoreLimit;
-        if (static_cast<uint32_t>(id) >= p.num_blocks) {
-            if (lane == 0) record_error(p.err, kErrBadBlockId);
-        } else {
-            const T* row = reinterpret_cast<const T*>(p.summary + static_cast<size_t>(id) * p.summary_stride) +
-                           (static_cast<size_t>(p.layer) * p.hkv + head) * 2 * p.D;
-            s = 0.0;
-            for (uint32_t e = lane; e < 2 * p.D; e += 32) s += static_cast<double>(to_float<T>(row[e])) * weight[e];
-            s = warp_sum(s);
+// The weights as three bf16 terms each, what the terms before leave of a
+// weight, rounded, and the size of the first: [4][PITCH].
+template <uint32_t PITCH>
+__device__ __forceinline__ void split_weights(const SelectParams& p, const double* weight, __nv_bfloat16* terms) {
+    for (uint32_t e = threadIdx.x; e < 2 * p.D; e += kSelThreads) {
+        double w = weight[e];
+#pragma unroll
+        for (int r = 0; r < 3; ++r) {
+            const __nv_bfloat16 term = __float2bfloat16_rn(static_cast<float>(w));
+            terms[r * PITCH + e] = term;
+            if (r == 0) terms[3 * PITCH + e] = __habs(term);
+            w -= static_cast<double>(__bfloat162float(term));
         }
-        if (lane == 0) score[i] = ordered_score(s);
+    }
+}
+
+// Scores one block after another, a warp each; lo and hi get their range. The
+// way of rows that 16-byte loads do not fit.
+template <typename T>
+__device__ __forceinline__ void score_each(const SelectParams& p, const SelectPart& part, float& lo, float& hi) {
+    for (uint32_t i = threadIdx.x >> 5; i < part.n; i += kSelWarps) {
+        const int32_t id = part.table[i];
+        double s = -kScoreLimit;
+        if (static_cast<uint32_t>(id) < p.num_blocks)
+            s = score_block<T>(p, id, part.head, part.weight);
+        else if ((threadIdx.x & 31) == 0)
+            record_error(p.err, kErrBadBlockId);
+        const float k = score_key(s);
+        if ((threadIdx.x & 31) == 0) {
+            part.score[i] = s;
+            part.key[i] = k;
+        }
+        lo = fminf(lo, k);
+        hi = fmaxf(hi, k);
     }
 }
 
 // The same with 16-byte loads: LANES lanes per block, VECS vectors a lane, and
-// UNROLL blocks of every lane group in flight. A lane keeps the weights of its
+// UNROLL blocks of every lane group per step. A lane keeps the weights of its
 // columns in registers, and the UNROLL partial sums of a group are reduced
 // together: each exchange halves the sums a lane carries.
 template <typename T, int LANES, int VECS>
-__device__ __forceinline__ void score_blocks_vec(const SelectParams& p, const int32_t* table, uint32_t head,
-                                                 const double* weight, uint32_t first, uint32_t n, double* score) {
+__device__ __forceinline__ void score_vectors(const SelectParams& p, const SelectPart& part, float& lo, float& hi) {
     constexpr int V = 16 / sizeof(T);
     constexpr int UNROLL = 8 / VECS;
     constexpr uint32_t kGroups = 32 / LANES;           // blocks of a warp-wide load
     constexpr uint32_t kStep = kGroups * UNROLL;       // blocks of a warp per step
     static_assert(kStep <= 32, "a lane holds one id of a step");
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t lane = threadIdx.x & 31, n = part.n;
     const uint32_t col = lane % LANES, group = lane / LANES;
     double w[VECS][V];
     bool live[VECS];
@@ -307,17 +589,17 @@ __device__ __forceinline__ void score_blocks_vec(const SelectParams& p, const in
         const uint32_t e = (col + j * LANES) * V;
         live[j] = e < 2 * p.D;
 #pragma unroll
-        for (int i = 0; i < V; ++i) w[j][i] = live[j] ? weight[e + i] : 0.0;
+        for (int i = 0; i < V; ++i) w[j][i] = live[j] ? part.weight[e + i] : 0.0;
     }
-    const T* rows = reinterpret_cast<const T*>(p.summary) + (static_cast<size_t>(p.layer) * p.hkv + head) * 2 * p.D +
-                    col * V;
+    const T* rows = reinterpret_cast<const T*>(p.summary) +
+                    (static_cast<size_t>(p.layer) * p.hkv + part.head) * 2 * p.D + col * V;
     const size_t stride = p.summary_stride / sizeof(T);
     auto ids_of = [&](uint32_t base) -> int32_t {
         const uint32_t i = base + lane;
-        return lane < kStep && i < n ? table[first + i] : 0;
+        return lane < kStep && i < n ? part.table[i] : 0;
     };
-    int32_t next = ids_of(warp * kStep);
-    for (uint32_t base = warp * kStep; base < n; base += kSelWarps * kStep) {
+    int32_t next = ids_of((threadIdx.x >> 5) * kStep);
+    for (uint32_t base = (threadIdx.x >> 5) * kStep; base < n; base += kSelWarps * kStep) {
         const int32_t ids = next;
         next = ids_of(base + kSelWarps * kStep);
         const bool bad = static_cast<uint32_t>(ids) >= p.num_blocks;
@@ -338,21 +620,22 @@ __device__ __forceinline__ void score_blocks_vec(const SelectParams& p, const in
             for (int j = 0; j < VECS; ++j)
                 if (live[j]) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) s[u] = fma(static_cast<double>(to_float<T>(x[u][j].v[i])), w[j][i], s[u]);
+                    for (int i = 0; i < V; ++i)
+                        s[u] = fma(static_cast<double>(to_float<T>(x[u][j].v[i])), w[j][i], s[u]);
                 }
         }
-        int live_sums = UNROLL;
+        int sums = UNROLL;
         uint32_t mine = 0;  // the sum this lane ends with
 #pragma unroll
         for (int off = LANES / 2; off > 0; off >>= 1) {
-            if (live_sums > 1) {
-                live_sums >>= 1;
+            if (sums > 1) {
+                sums >>= 1;
 #pragma unroll
                 for (int u = 0; u < UNROLL / 2; ++u) {
-                    if (u < live_sums) {
+                    if (u < sums) {
                         const bool upper = lane & off;
-                        const double send = upper ? s[u] : s[u + live_sums];
-                        s[u] = (upper ? s[u + live_sums] : s[u]) + __shfl_xor_sync(0xffffffffu, send, off);
+                        const double send = upper ? s[u] : s[u + sums];
+                        s[u] = (upper ? s[u + sums] : s[u]) + __shfl_xor_sync(0xffffffffu, send, off);
                     }
                 }
                 mine = mine * 2 + ((lane & off) ? 1 : 0);
@@ -363,18 +646,145 @@ __device__ __forceinline__ void score_blocks_vec(const SelectParams& p, const in
         constexpr uint32_t kSame = LANES / UNROLL;  // lanes that end with the same sum
         const bool skip = __shfl_sync(0xffffffffu, bad, mine * kGroups + group);
         const uint32_t i = base + mine * kGroups + group;
-        if (lane % kSame == 0 && i < n) score[i] = skip ? -kScoreLimit : ordered_score(s[0]);
+        if (i < n) {
+            const double sum = skip ? -kScoreLimit : ordered_score(s[0]);
+            const float k = score_key(sum);
+            if (lane % kSame == 0) {
+                part.score[i] = sum;
+                part.key[i] = k;
+            }
+            lo = fminf(lo, k);
+            hi = fmaxf(hi, k);
+        }
     }
 }
 
-// LANES = 0: one element at a time.
+// bf16 rows of LOADS * 32 elements (head_dim = 16 LOADS) on the tensor cores,
+// 16 blocks of a warp per step: the rows are the A operand of m16n8k16, read
+// from global memory straight into its fragments (lane l holds part l % 4 of
+// blocks l / 4 and l / 4 + 8), and the weights, as three bf16 terms in three
+// columns, are B. The order of k does not matter to a product, so a lane's 16
+// bytes are two k steps.
+//
+// Error: three terms leave 2^-24 of a weight; the 32 LOADS products of each are
+// summed in 32 bits, an addition off by at most 2^-23 of the sum of their
+// sizes. Twice that, LOADS 2^-17, times sum_d |w_d x_d| bounds a score's error.
+// That sum is a product as well: the sizes of the weights, in a fourth column
+// of B, by the sizes of the row; its largest is `top` (infinite or NaN where a
+// row or a weight is, or is more than 32 bits hold). Returns the factor.
+template <int LOADS>
+__device__ __forceinline__ double score_tiles(const SelectParams& p, const SelectPart& part, uint32_t b, double* weight,
+                                              __nv_bfloat16* terms, float& lo, float& hi, float& top) {
+    using T = __nv_bfloat16;
+    constexpr uint32_t kPitch = 32 * LOADS + 8;  // elements between terms: their rows fall in different banks
+    constexpr uint32_t kStride = kSelWarps * 16;
+    const uint32_t lane = threadIdx.x & 31, n = part.n;
+    const uint32_t row = lane >> 2, col = lane & 3;
+    const T* rows = reinterpret_cast<const T*>(p.summary) +
+                    (static_cast<size_t>(p.layer) * p.hkv + part.head) * 2 * p.D + col * 8;
+    const size_t stride = p.summary_stride / sizeof(T);
+    // a step past the end repeats its last block
+    auto id_of = [&](uint32_t i) { return i < n + kStride ? part.table[min(i, n - 1)] : 0; };
+    uint32_t base = (threadIdx.x >> 5) * 16;
+    int32_t id0 = 0, id1 = 0;
+    if (base < n) {
+        id0 = id_of(base + row);
+        id1 = id_of(base + row + 8);
+    }
+    make_weights<T>(p, b, part.head, weight);
+    __syncthreads();
+    split_weights<kPitch>(p, weight, terms);
+    __syncthreads();
+    const T* columns = terms + row * kPitch + col * 8;
+#pragma unroll 1
+    for (; base < n; base += kStride) {
+        const bool bad0 = static_cast<uint32_t>(id0) >= p.num_blocks, bad1 = static_cast<uint32_t>(id1) >= p.num_blocks;
+        if (bad0 || bad1) record_error(p.err, kErrBadBlockId);
+        const T* at0 = rows + static_cast<size_t>(bad0 ? 0 : id0) * stride;
+        const T* at1 = rows + static_cast<size_t>(bad1 ? 0 : id1) * stride;
+        uint4 x[LOADS], y[LOADS];
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            x[j] = *reinterpret_cast<const uint4*>(at0 + j * 32);
+            y[j] = *reinterpret_cast<const uint4*>(at1 + j * 32);
+        }
+        id0 = id_of(base + kStride + row);
+        id1 = id_of(base + kStride + row + 8);
+        float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+        float size_even[4] = {0.f, 0.f, 0.f, 0.f}, size_odd[4] = {0.f, 0.f, 0.f, 0.f};
+        constexpr uint32_t kSize = 0x7fff7fffu;
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const uint4 w = row < 4 ? *reinterpret_cast<const uint4*>(columns + j * 32) : make_uint4(0, 0, 0, 0);
+            const uint4 u = x[j], v = y[j];
+            mma_bf16_16816(even, {u.x, v.x, u.y, v.y}, w.x, w.y);
+            mma_bf16_16816(odd, {u.z, v.z, u.w, v.w}, w.z, w.w);
+            mma_bf16_16816(size_even, {u.x & kSize, v.x & kSize, u.y & kSize, v.y & kSize}, w.x, w.y);
+            mma_bf16_16816(size_odd, {u.z & kSize, v.z & kSize, u.w & kSize, v.w & kSize}, w.z, w.w);
+        }
+        // columns 0 and 1 are in the lanes with col 0, 2 and 3 in those with col 1
+        if (col == 1) top = max_nan(top, max_nan(size_even[1] + size_odd[1], size_even[3] + size_odd[3]));
+        float s0 = even[0] + odd[0], s1 = even[2] + odd[2];
+        s0 += (even[1] + odd[1]) + __shfl_down_sync(0xffffffffu, s0, 1);
+        s1 += (even[3] + odd[3]) + __shfl_down_sync(0xffffffffu, s1, 1);
+        if (col == 0) {
+            const uint32_t i = base + row;
+            const float k0 = bad0 ? -kKeyLimit : ordered_key(s0), k1 = bad1 ? -kKeyLimit : ordered_key(s1);
+            if (i < n) {
+                part.key[i] = k0;
+                lo = fminf(lo, k0);
+                hi = fmaxf(hi, k0);
+            }
+            if (i + 8 < n) {
+                part.key[i + 8] = k1;
+                lo = fminf(lo, k1);
+                hi = fmaxf(hi, k1);
+            }
+        }
+    }
+    return LOADS * 0x1p-17;
+}
+
+// How a kernel scores: one element at a time, in vectors of LANES x VECS, or
+// in tiles of LOADS x 16 dimensions.
+struct ByElement {};
+template <int LANES, int VECS>
+struct ByVector {};
+template <int LOADS>
+struct ByTile {};
+
+// Scores of a part, its weights made on the way; returns their error factor.
+template <typename T>
+__device__ __forceinline__ double score_part(ByElement, const SelectParams& p, const SelectPart& part, uint32_t b,
+                                             double* weight, float& lo, float& hi, float&) {
+    make_weights<T>(p, b, part.head, weight);
+    __syncthreads();
+    score_each<T>(p, part, lo, hi);
+    return 0.0;
+}
 template <typename T, int LANES, int VECS>
-__global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p) {
+__device__ __forceinline__ double score_part(ByVector<LANES, VECS>, const SelectParams& p, const SelectPart& part,
+                                             uint32_t b, double* weight, float& lo, float& hi, float&) {
+    make_weights<T>(p, b, part.head, weight);
+    __syncthreads();
+    score_vectors<T, LANES, VECS>(p, part, lo, hi);
+    return 0.0;
+}
+template <typename T, int LOADS>
+__device__ __forceinline__ double score_part(ByTile<LOADS>, const SelectParams& p, const SelectPart& part, uint32_t b,
+                                             double* weight, float& lo, float& hi, float& top) {
+    __shared__ __align__(16) __nv_bfloat16 terms[4 * (32 * LOADS + 8)];
+    return score_tiles<LOADS>(p, part, b, weight, terms, lo, hi, top);
+}
+
+template <typename T, typename How>
+__global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectParams p) {
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ SelectShared s;
     double* weight = reinterpret_cast<double*>(dyn);  // [down D | up D], against [min D | max D]
     double* score = weight + 2 * p.D;
-    uint8_t* state = reinterpret_cast<uint8_t*>(score + p.chunk);
+    float* key = reinterpret_cast<float*>(score + p.chunk);
+    uint8_t* state = reinterpret_cast<uint8_t*>(key + p.chunk);
 
     wait_for_previous_kernel();
     allow_next_kernel();
@@ -392,70 +802,43 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
             out[i] = i < blocks ? static_cast<int32_t>(i) : -1;
         return;
     }
-    for (uint32_t d = threadIdx.x; d < p.D; d += kSelThreads) {
-        const T* q = static_cast<const T*>(p.q) + b * p.q_pitch + static_cast<size_t>(head) * p.group * p.D + d;
-        double up = 0.0, down = 0.0;
-        for (uint32_t g = 0; g < p.group; ++g) {
-            const double x = static_cast<double>(to_float<T>(q[static_cast<size_t>(g) * p.D]));
-            // a NaN goes to both sums
-            if (!(x < 0.0)) up += x;
-            if (!(x > 0.0)) down += x;
-        }
-        weight[d] = down;
-        weight[p.D + d] = up;
-    }
     // blocks between sink and recent, this CTA's part of them
     const uint32_t end = blocks - p.recent;
     const uint32_t part = (end - p.sink + cluster - 1) / cluster;
     const uint32_t first = min(p.sink + rank * part, end);
     const uint32_t n = min(part, end - first);
     const uint32_t need = p.keep - p.sink - p.recent;
-    for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) state[i] = need > 0 ? kOpen : kDropped;
-    __syncthreads();
-    if (need > 0) {
-        const int32_t* table = p.tables + static_cast<size_t>(b) * p.pitch;
-        if constexpr (LANES == 0)
-            score_blocks<T>(p, table, head, weight, first, n, score);
-        else
-            score_blocks_vec<T, LANES, VECS>(p, table, head, weight, first, n, score);
-        __syncthreads();
-        take_best(score, state, n, first, need, s, cluster, rank);
-    }
-    // ascending list: sink, what the ranks took in rank order, recent
-    uint32_t mine = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += kSelThreads) mine += state[i] == kTaken;
-    const uint32_t taken = cta_count(mine, s);
-    if (threadIdx.x == 0) s.taken = taken;
-    cluster_barrier(cluster);
-    uint32_t at = p.sink;
-    for (uint32_t r = 0; r < rank; ++r) at += *of_rank(&s.taken, cluster, r);
-    for (uint32_t i0 = 0; i0 < n; i0 += kSelThreads) {
-        const uint32_t i = i0 + threadIdx.x;
-        const bool is = i < n && state[i] == kTaken;
-        const uint32_t votes = __ballot_sync(0xffffffffu, is);
-        if ((threadIdx.x & 31) == 0) s.warp_sum[threadIdx.x >> 5] = __popc(votes);
-        __syncthreads();
-        uint32_t to = at + __popc(votes & ((1u << (threadIdx.x & 31)) - 1u));
-        for (uint32_t w = 0; w < kSelWarps; ++w) {
-            if (w < (threadIdx.x >> 5)) to += s.warp_sum[w];
-            at += s.warp_sum[w];
-        }
-        if (is) out[to] = static_cast<int32_t>(first + i);
-        __syncthreads();
-    }
     if (rank == 0)
         for (uint32_t i = threadIdx.x; i < p.sink; i += kSelThreads) out[i] = static_cast<int32_t>(i);
     if (rank == cluster - 1)
         for (uint32_t i = threadIdx.x; i < p.recent; i += kSelThreads)
             out[p.keep - p.recent + i] = static_cast<int32_t>(end + i);
+    if (need == 0) return;  // the whole cluster
+
+    const SelectPart work = {p.tables + static_cast<size_t>(b) * p.pitch + first, weight, key, score, state, first, n, head,
+                             rank};
+    float lo = INFINITY, hi = -INFINITY, top = 0.f;
+    const double error_scale = score_part<T>(How{}, p, work, b, weight, lo, hi, top);
+    __syncthreads();
+    const uint32_t before = take_best<T>(p, work, need, lo, hi, top, error_scale, s);
+
+    // ascending list: what the ranks took, in rank order, a run of blocks per thread
+    const uint32_t per = (n + kSelThreads - 1) / kSelThreads;
+    const uint32_t run = min(threadIdx.x * per, n), stop = min(run + per, n);
+    uint32_t mine = 0;
+    for (uint32_t i = run; i < stop; ++i) mine += state[i] == kTaken;
+    uint32_t all;
+    int32_t* to = out + p.sink + before + cta_scan(mine, all, s);
+    for (uint32_t i = run; i < stop; ++i)
+        if (state[i] == kTaken) *to++ = static_cast<int32_t>(first + i);
     // no CTA leaves while another may read its shared memory
-    cluster_barrier(cluster);
+    if (cluster > 1) cg::this_cluster().barrier_wait();
 }
 
-template <typename T, int LANES, int VECS>
-int launch_select_t(const SelectParams& p, uint32_t segments, size_t smem, cudaStream_t st) {
+template <typename T, typename How>
+int launch_select_t(How, const SelectParams& p, uint32_t segments, size_t smem, cudaStream_t st) {
     static std::atomic<std::uint64_t> attr_done{0};
-    auto kern = select_kernel<T, LANES, VECS>;
+    auto kern = select_kernel<T, How>;
     const int rc = set_smem_limit_once(attr_done, reinterpret_cast<const void*>(kern), 200 * 1024,
                                        "cudaFuncSetAttribute(select_blocks)");
     if (rc != QVP_OK) return rc;
@@ -466,15 +849,20 @@ int launch_select_t(const SelectParams& p, uint32_t segments, size_t smem, cudaS
 template <typename T>
 int launch_select(const SelectParams& p, uint32_t segments, size_t smem, cudaStream_t st) {
     constexpr uint32_t V = 16 / sizeof(T);
-    const uint32_t vectors = 2 * p.D / V;
     if (p.D % V != 0 || !aligned_to(p.summary, 16) || p.summary_stride % 16 != 0)
-        return launch_select_t<T, 0, 1>(p, segments, smem, st);
-    if (vectors <= 16) return launch_select_t<T, 16, 1>(p, segments, smem, st);
-    if (vectors <= 32) return launch_select_t<T, 32, 1>(p, segments, smem, st);
-    if constexpr (sizeof(T) == 4) {
-        if (vectors > 64) return launch_select_t<T, 32, 4>(p, segments, smem, st);
+        return launch_select_t<T>(ByElement{}, p, segments, smem, st);
+    if constexpr (sizeof(T) == 2) {
+        if (p.D == 64) return launch_select_t<T>(ByTile<4>{}, p, segments, smem, st);
+        if (p.D == 96) return launch_select_t<T>(ByTile<6>{}, p, segments, smem, st);
+        if (p.D == 128) return launch_select_t<T>(ByTile<8>{}, p, segments, smem, st);
     }
-    return launch_select_t<T, 32, 2>(p, segments, smem, st);
+    const uint32_t vectors = 2 * p.D / V;
+    if (vectors <= 16) return launch_select_t<T>(ByVector<16, 1>{}, p, segments, smem, st);
+    if (vectors <= 32) return launch_select_t<T>(ByVector<32, 1>{}, p, segments, smem, st);
+    if constexpr (sizeof(T) == 4) {
+        if (vectors > 64) return launch_select_t<T>(ByVector<32, 4>{}, p, segments, smem, st);
+    }
+    return launch_select_t<T>(ByVector<32, 2>{}, p, segments, smem, st);
 }
 
 }  // namespace
@@ -539,15 +927,19 @@ extern "C" int qvp_select_blocks(const qvp_select_args* args, qvp_stream_t strea
     const uint32_t blocks = ceil_div(a.max_context_len, sh.tokens_per_block);
     const uint32_t scored = blocks > a.max_selected ? blocks - a.sink_blocks - a.recent_blocks : 0;
     const uint64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
+    // Two CTAs are resident per SM: share a list of scores while the whole grid
+    // still is (256 rows of 2048 blocks: 52.9 us with one CTA a row, 65.6 with
+    // two; 8 rows: 23.2 with one, 12.6 with eight), and as far as they have to
+    // to hold it.
     p.cluster = 1;
-    while (p.cluster < kSelMaxCluster &&
-           (ceil_div(scored, p.cluster) > kSelMaxChunk || (segments * p.cluster < 2 * sms && scored / p.cluster > 64)))
+    while (p.cluster < kSelMaxCluster && (ceil_div(scored, p.cluster) > kSelMaxChunk ||
+                                          (segments * p.cluster <= sms && scored / p.cluster > 64)))
         p.cluster *= 2;
     p.chunk = static_cast<uint32_t>(round_up(ceil_div(scored, p.cluster), 16));
     if (p.chunk > kSelMaxChunk)
         return fail(QVP_ERR_UNSUPPORTED, "contexts of more than %u blocks", kSelMaxChunk * kSelMaxCluster);
     if (segments * p.cluster > 0x7fffffffu) return fail(QVP_ERR_UNSUPPORTED, "more than 2^31 sequences and heads");
-    const size_t smem = 2 * sizeof(double) * p.D + static_cast<size_t>(p.chunk) * (sizeof(double) + 1);
+    const size_t smem = 2 * sizeof(double) * p.D + static_cast<size_t>(p.chunk) * (sizeof(double) + sizeof(float) + 1);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return a.dtype == QVP_DTYPE_F32 ? launch_select<float>(p, static_cast<uint32_t>(segments), smem, st)
                                     : launch_select<__nv_bfloat16>(p, static_cast<uint32_t>(segments), smem, st);
