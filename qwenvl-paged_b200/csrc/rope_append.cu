@@ -10,17 +10,18 @@
 // Every q, k and v element is read once and written once: the call is bound
 // by HBM for prompts and by latency for single tokens. A CTA takes the new
 // tokens of one cache block (so a block's summary belongs to one CTA) and
-// either its K and V or some of its query heads; it makes the cosines and
-// sines of its tokens once, in shared memory, for all its heads.
+// either its K and V or some of its query heads. It makes the cosines and sines
+// of its tokens once for all heads, in shared memory; then each thread goes
+// through the heads with those of its run of pairs of one token in registers.
 #include "sparse_common.cuh"
 
 namespace qvp {
 
 namespace {
 
-constexpr int kRopeThreads = 256;
-constexpr int kRopeTokens = 16;       // tokens whose cosines and sines are held at once
-constexpr int kMaxPairs = 128;        // head_dim <= 256
+constexpr int kRopeThreads = 128;
+constexpr uint32_t kRopeTokens = 16;  // most tokens of a CTA at a time
+constexpr uint32_t kMaxPairs = 128;   // head_dim <= 256
 
 struct RopeParams {
     uint8_t* pool;
@@ -46,17 +47,22 @@ struct RopeParams {
     uint32_t batch, max_q;
     uint32_t units;          // cache blocks a sequence's new tokens can touch
     uint32_t heads_per_cta;  // query heads of a CTA with blockIdx.y > 0
+    uint32_t tokens;         // tokens of a CTA at a time
     uint32_t rotary;
     bool interleaved;
     uint32_t section_end[QVP_ROPE_MAX_AXES];
 };
 
-// cos and sin of pos * f. The angle is taken modulo a turn in 64 bits, where
-// a position of 2^31 still leaves 2^-22 of a turn; what is left is below half
-// a turn, and 32 bits hold it.
-__device__ __forceinline__ float2 turn(int32_t pos, float f) {
+// Turns per position of a pair, in 64 bits, and cos and sin of the angle at
+// `pos`: it is taken modulo a turn in 64 bits, where a position of 2^31 still
+// leaves 2^-21 of a turn; what is left is below half a turn, and 32 bits hold
+// it.
+__device__ __forceinline__ double turns_of(float f) {
     constexpr double kInvTwoPi = 0.15915494309189533576888376337251;
-    const double turns = static_cast<double>(pos) * static_cast<double>(f) * kInvTwoPi;
+    return static_cast<double>(f) * kInvTwoPi;
+}
+__device__ __forceinline__ float2 turn(int32_t pos, double per_pos) {
+    const double turns = static_cast<double>(pos) * per_pos;
     const float part = static_cast<float>(2.0 * (turns - rint(turns)));
     float2 cs;
     sincospif(part, &cs.y, &cs.x);
@@ -85,42 +91,83 @@ struct Item {
     }
 };
 
-// cs: cos and sin of the item's first pair. Products and their sum are 32-bit;
+// The elements of a vector as floats and back, each rounded once.
+template <typename T, int VEC>
+__device__ __forceinline__ void to_floats(const Vec<T, VEC>& a, float* x) {
+    if constexpr (sizeof(T) == 2 && VEC > 1) {
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(&a)[j];
+            x[2 * j] = __uint_as_float(w << 16);
+            x[2 * j + 1] = __uint_as_float(w & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[j] = to_float<T>(a.v[j]);
+    }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void from_floats(const float* x, Vec<T, VEC>& a) {
+    if constexpr (sizeof(T) == 2 && VEC > 1) {
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) reinterpret_cast<uint32_t*>(&a)[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) a.v[j] = from_float<T>(x[j]);
+    }
+}
+
+// cs: cosines and sines of the item's pairs. Products and their sum are 32-bit;
 // the result is rounded to T once.
 template <typename T, int VEC>
-__device__ __forceinline__ void rotate(Vec<T, VEC>& a, Vec<T, VEC>& b, const float2* cs, bool interleaved) {
-    float x[VEC], y[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        const float u = to_float<T>(a.v[j]), w = to_float<T>(b.v[j]);
-        x[j] = u;
-        y[j] = w;
-    }
+__device__ __forceinline__ void rotate(Vec<T, VEC>& a, Vec<T, VEC>& b, const float2 (&cs)[VEC], bool interleaved) {
+    float x[2 * VEC];
+    to_floats<T, VEC>(a, x);
+    to_floats<T, VEC>(b, x + VEC);
     if (VEC > 1 && interleaved) {
-        float flat[2 * VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            flat[j] = x[j];
-            flat[VEC + j] = y[j];
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float2 c = cs[j];
-            const float u = flat[2 * j], w = flat[2 * j + 1];
-            flat[2 * j] = u * c.x - w * c.y;
-            flat[2 * j + 1] = w * c.x + u * c.y;
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            a.v[j] = from_float<T>(flat[j]);
-            b.v[j] = from_float<T>(flat[VEC + j]);
+            const float u = x[2 * j], w = x[2 * j + 1];
+            x[2 * j] = u * cs[j].x - w * cs[j].y;
+            x[2 * j + 1] = w * cs[j].x + u * cs[j].y;
         }
     } else {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            const float2 c = cs[j];
-            a.v[j] = from_float<T>(x[j] * c.x - y[j] * c.y);
-            b.v[j] = from_float<T>(y[j] * c.x + x[j] * c.y);
+            const float u = x[j], w = x[VEC + j];
+            x[j] = u * cs[j].x - w * cs[j].y;
+            x[VEC + j] = w * cs[j].x + u * cs[j].y;
+        }
+    }
+    from_floats<T, VEC>(x, a);
+    from_floats<T, VEC>(x + VEC, b);
+}
+
+// Turns (or copies) one item of heads [0, count) of a token, every step-th
+// from `first` on: rows src + h * D to dst + h * D.
+template <typename T, int VEC>
+__device__ __forceinline__ void turn_heads(const T* src, T* dst, uint32_t first, uint32_t count, uint32_t step,
+                                           uint32_t D, const Item<VEC>& x, const float2 (&cs)[VEC], bool interleaved) {
+    constexpr int kFlight = 2;  // heads whose loads are in flight together
+    const bool two = x.e1 < D;
+    for (uint32_t h0 = first; h0 < count; h0 += kFlight * step) {
+        Vec<T, VEC> u[kFlight], w[kFlight];
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            const uint32_t h = h0 + k * step;
+            if (h < count) {
+                u[k] = load_vec<T, VEC>(src + h * D + x.e0);
+                if (two) w[k] = load_vec<T, VEC>(src + h * D + x.e1);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+            const uint32_t h = h0 + k * step;
+            if (h < count) {
+                if (x.turned) rotate<T, VEC>(u[k], w[k], cs, interleaved);
+                store_vec<T, VEC>(dst + h * D + x.e0, u[k]);
+                if (two) store_vec<T, VEC>(dst + h * D + x.e1, w[k]);
+            }
         }
     }
 }
@@ -129,7 +176,9 @@ __device__ __forceinline__ void rotate(Vec<T, VEC>& a, Vec<T, VEC>& b, const flo
 // else one by one. grid (batch * units, 1 + groups of query heads).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeParams p) {
-    __shared__ float2 cs[kRopeTokens * kMaxPairs];
+    // of pair it * VEC + j of token t at [j][t * row_items + it], rows one apart
+    // from a multiple of the banks
+    __shared__ float2 table[kRopeTokens * kMaxPairs + VEC];
     // partial ranges of the token groups of K, two vectors each
     __shared__ Vec<T, VEC> part[kRopeThreads][4];
 
@@ -162,75 +211,66 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
         frame = p.pool + static_cast<size_t>(id) * p.block_stride;
     }
     const uint32_t D = p.D;
-    const uint32_t half = p.rotary / 2;
     const uint32_t row_items = (D + 2 * VEC - 1) / (2 * VEC);
     const size_t slot_elems = static_cast<size_t>(p.hkv) * D;                   // elements of one token's K or V
     T* kslots = reinterpret_cast<T*>(frame) + static_cast<size_t>(p.layer) * 2 * p.T * slot_elems;
     T* vslots = kslots + p.T * slot_elems;
-    const size_t row0 = static_cast<size_t>(b) * p.max_q;
-
-    // K: a thread owns one item of one kv head and every groups-th token
-    const uint32_t k_items = p.hkv * row_items;
-    uint32_t groups = 1;
-    while (groups < kRopeTokens && groups * 2 * k_items <= kRopeThreads) groups *= 2;
-    const uint32_t h0 = kv ? 0u : (blockIdx.y - 1) * p.heads_per_cta;
+    const size_t row0 = static_cast<size_t>(b) * p.max_q + (lo - first);        // token row of position lo
+    const uint32_t cnt = hi - lo;
+    const uint32_t half = p.rotary / 2;
+    const uint32_t h0 = kv ? 0 : (blockIdx.y - 1) * p.heads_per_cta;
     const uint32_t nh = kv ? p.hkv : min(p.heads_per_cta, p.hq - h0);
-
-    for (uint32_t t0 = lo; t0 < hi; t0 += kRopeTokens) {
-        const uint32_t cnt = min(static_cast<uint32_t>(kRopeTokens), hi - t0);
-        const uint32_t row = t0 - first;                                        // token row of t0
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < cnt * half; i += kRopeThreads) {
-            const uint32_t t = i / half, pr = i % half;
-            int32_t pos = static_cast<int32_t>(t0 + t);
-            if (p.pos != nullptr) {
-                uint32_t axis = 0;
-                while (pr >= p.section_end[axis]) ++axis;                       // the last end is half
-                pos = p.pos[(static_cast<size_t>(axis) * p.batch + b) * p.max_q + row + t];
+    const T* src = kv ? static_cast<const T*>(p.k) + row0 * p.k_pitch
+                      : static_cast<const T*>(p.q) + row0 * p.q_pitch + static_cast<size_t>(h0) * D;
+    const size_t src_pitch = kv ? p.k_pitch : p.q_pitch;
+    T* dst = kv ? kslots + (lo - base) * slot_elems
+                : static_cast<T*>(p.q_out) + (row0 * p.hq + h0) * static_cast<size_t>(D);
+    const size_t dst_pitch = kv ? slot_elems : static_cast<size_t>(p.hq) * D;
+    const T* v = static_cast<const T*>(p.v) + row0 * p.v_pitch;
+    // a thread's place: an item of a token, and the heads it shares with the
+    // threads at the same place
+    const uint32_t places = p.tokens * row_items;
+    const uint32_t sharers = places < kRopeThreads ? kRopeThreads / places : 1;
+    // the pair whose angles a thread makes, for every at_once-th token
+    const uint32_t at_once = half > 0 ? kRopeThreads / half : 0;
+    const uint32_t pair = half > 0 ? threadIdx.x % half : 0;
+    const double per_pos = half > 0 ? turns_of(p.inv_freq[pair]) : 0.0;
+    const int32_t* positions = nullptr;
+    if (p.pos != nullptr) {
+        uint32_t axis = 0;
+        while (pair >= p.section_end[axis]) ++axis;                             // the last end is rotary / 2
+        positions = p.pos + static_cast<size_t>(axis) * p.batch * p.max_q + row0;
+    }
+    for (uint32_t t0 = 0; t0 < cnt; t0 += p.tokens) {
+        const uint32_t some = min(p.tokens, cnt - t0);
+        if (t0 > 0) __syncthreads();
+        if (threadIdx.x < at_once * half) {
+#pragma unroll 4
+            for (uint32_t t = threadIdx.x / half; t < some; t += at_once) {
+                const int32_t at = positions != nullptr ? positions[t0 + t] : static_cast<int32_t>(lo + t0 + t);
+                table[pair % VEC * (places + 1) + t * row_items + pair / VEC] = turn(at, per_pos);
             }
-            cs[t * half + pr] = turn(pos, p.inv_freq[pr]);
         }
         __syncthreads();
-        if (!kv) {
-            const T* q = static_cast<const T*>(p.q);
-            T* out = static_cast<T*>(p.q_out);
-            const uint32_t total = cnt * nh * row_items;
-            for (uint32_t i = threadIdx.x; i < total; i += kRopeThreads) {
-                const uint32_t t = i / (nh * row_items), r = i % (nh * row_items);
-                const uint32_t h = h0 + r / row_items, it = r % row_items;
-                const Item<VEC> x(it, p.rotary, p.interleaved);
-                const T* src = q + (row0 + row + t) * p.q_pitch + static_cast<size_t>(h) * D;
-                T* dst = out + ((row0 + row + t) * p.hq + h) * D;
-                Vec<T, VEC> u = load_vec<T, VEC>(src + x.e0), w;
-                const bool two = x.e1 < D;
-                if (two) w = load_vec<T, VEC>(src + x.e1);
-                if (x.turned) rotate<T, VEC>(u, w, cs + t * half + it * VEC, p.interleaved);
-                store_vec<T, VEC>(dst + x.e0, u);
-                if (two) store_vec<T, VEC>(dst + x.e1, w);
+        for (uint32_t i = threadIdx.x; i < places * sharers; i += kRopeThreads) {
+            const uint32_t it = i % row_items, t = i / row_items % p.tokens;
+            if (t >= some) continue;
+            const Item<VEC> x(it, p.rotary, p.interleaved);
+            float2 cs[VEC];
+            if (x.turned) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) cs[j] = table[j * (places + 1) + t * row_items + it];
             }
-            continue;
+            turn_heads<T, VEC>(src + (t0 + t) * src_pitch, dst + (t0 + t) * dst_pitch, i / places, nh, sharers, D, x, cs,
+                               p.interleaved);
         }
-        const T* v = static_cast<const T*>(p.v);
+    }
+    if (kv) {
         const uint32_t v_items = static_cast<uint32_t>(slot_elems / VEC);
+#pragma unroll 4
         for (uint32_t i = threadIdx.x; i < cnt * v_items; i += kRopeThreads) {
             const uint32_t t = i / v_items, e = (i % v_items) * VEC;
-            store_vec<T, VEC>(vslots + (t0 - base + t) * slot_elems + e,
-                              load_vec<T, VEC>(v + (row0 + row + t) * p.v_pitch + e));
-        }
-        const T* k = static_cast<const T*>(p.k);
-        for (uint32_t i = threadIdx.x; i < groups * k_items; i += kRopeThreads) {
-            const uint32_t g = i / k_items, h = (i % k_items) / row_items, it = i % row_items;
-            const Item<VEC> x(it, p.rotary, p.interleaved);
-            const bool two = x.e1 < D;
-            for (uint32_t t = g; t < cnt; t += groups) {
-                const T* src = k + (row0 + row + t) * p.k_pitch + static_cast<size_t>(h) * D;
-                T* dst = kslots + (t0 - base + t) * slot_elems + static_cast<size_t>(h) * D;
-                Vec<T, VEC> u = load_vec<T, VEC>(src + x.e0), w;
-                if (two) w = load_vec<T, VEC>(src + x.e1);
-                if (x.turned) rotate<T, VEC>(u, w, cs + t * half + it * VEC, p.interleaved);
-                store_vec<T, VEC>(dst + x.e0, u);
-                if (two) store_vec<T, VEC>(dst + x.e1, w);
-            }
+            store_vec<T, VEC>(vslots + (lo - base + t) * slot_elems + e, load_vec<T, VEC>(v + t * p.v_pitch + e));
         }
     }
     if (!kv || p.summary == nullptr) return;
@@ -239,6 +279,10 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
     // writes are visible to it after the barrier.
     __syncthreads();
     const uint32_t filled = min(p.T, static_cast<uint32_t>(ctx) - base);
+    // a thread owns one item of one kv head and every groups-th slot
+    const uint32_t k_items = p.hkv * row_items;
+    uint32_t groups = 1;
+    while (groups < kRopeTokens && groups * 2 * k_items <= kRopeThreads) groups *= 2;
     T* bounds = reinterpret_cast<T*>(p.summary + static_cast<size_t>(id) * p.summary_stride) +
                 static_cast<size_t>(p.layer) * 2 * slot_elems;
     for (uint32_t i0 = 0; i0 < groups * k_items; i0 += kRopeThreads) {
@@ -393,8 +437,15 @@ extern "C" int qvp_rope_append(const qvp_rope_append_args* args, qvp_stream_t st
     p.units = p.units < a.max_blocks_per_seq ? p.units : a.max_blocks_per_seq;
     if (static_cast<uint64_t>(p.units) * a.batch > 0x7fffffffu)
         return fail(QVP_ERR_UNSUPPORTED, "more than 2^31 blocks in one call");
-    p.heads_per_cta = 8;
-    const uint32_t groups = a.num_query_heads > 0 ? ceil_div(a.num_query_heads, p.heads_per_cta) : 0;
+    p.tokens = 1;
+    while (p.tokens < kRopeTokens && p.tokens < a.max_query_len) p.tokens *= 2;
+    // All query heads of a token in one CTA share its cosines; they are split
+    // while the grid would leave SMs without work.
+    const uint64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
+    uint32_t groups = a.num_query_heads > 0 ? 1 : 0;
+    while (groups * 4 < a.num_query_heads && static_cast<uint64_t>(p.units) * a.batch * groups < 4 * sms) groups *= 2;
+    p.heads_per_cta = groups > 0 ? ceil_div(a.num_query_heads, groups) : 0;
+    if (groups > 0) groups = ceil_div(a.num_query_heads, p.heads_per_cta);
     const dim3 grid(p.units * a.batch, 1 + groups);
 
     const uint32_t V = 16 / elem;
