@@ -20,6 +20,13 @@ namespace qvp {
 
 namespace {
 
+constexpr uint32_t kMaxCluster = 8;
+
+// Weight of a partial result whose maximum is m in one whose maximum is M.
+// Without a score above -inf its sums are 0, or NaN from a NaN score, and stay
+// as they are.
+__device__ __forceinline__ float partial_weight(float m, float M) { return m == -INFINITY ? 1.f : exp2f(m - M); }
+
 struct SelectedParams {
     const uint8_t* pool;
     size_t block_stride;
@@ -36,6 +43,7 @@ struct SelectedParams {
     uint32_t T, layer, num_layers, hq, hkv, D, group;
     uint32_t keep;
     uint32_t cluster;  // CTAs that share a (sequence, kv head)
+    uint32_t round;    // listed slots a warp takes at a time (any shape)
     float scale_log2;  // scale * log2(e): the softmax is computed in powers of two
 };
 
@@ -61,7 +69,6 @@ struct SelectedParams {
 
 constexpr int kTileWarps = 4;
 constexpr int kTileThreads = kTileWarps * 32;
-constexpr uint32_t kTileMaxCluster = 8;
 
 template <int D, int STAGES>
 struct TileShape {
@@ -324,8 +331,6 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         const float inv = 1.f / sum;
         *reinterpret_cast<uint32_t*>(out + g * D + d) = any != 0 ? pack_bf16x2(x * inv, y * inv) : 0u;
     };
-    // without a score above -inf a partial's sums are 0, or NaN from a NaN score
-    auto weight_of = [](float m, float M) { return m == -INFINITY ? 1.f : exp2f(m - M); };
     for (uint32_t i = threadIdx.x; i < static_cast<uint32_t>(G) * (D / 2); i += kTileThreads) {
         const uint32_t g = i / (D / 2), d = i % (D / 2) * 2;
         float M = -INFINITY;
@@ -335,7 +340,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 #pragma unroll
         for (int w = 0; w < kTileWarps; ++w) {
             const float2 o = *reinterpret_cast<const float2*>(smem + w * S::kRing + (g * D + d) * 4);
-            const float weight = weight_of(stats[w * 36 + g], M);
+            const float weight = partial_weight(stats[w * 36 + g], M);
             sum += weight * stats[w * 36 + 16 + g];
             x += weight * o.x;
             y += weight * o.y;
@@ -358,11 +363,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     for (uint32_t i = rank * kTileThreads + threadIdx.x; i < static_cast<uint32_t>(G) * (D / 2);
          i += cluster * kTileThreads) {
         const uint32_t g = i / (D / 2), d = i % (D / 2) * 2;
-        float m[kTileMaxCluster], l[kTileMaxCluster];
-        float2 o[kTileMaxCluster];
+        float m[kMaxCluster], l[kMaxCluster];
+        float2 o[kMaxCluster];
         float M = -INFINITY;
 #pragma unroll
-        for (uint32_t r = 0; r < kTileMaxCluster; ++r) {
+        for (uint32_t r = 0; r < kMaxCluster; ++r) {
             m[r] = -INFINITY;
             l[r] = 0.f;
             o[r] = make_float2(0.f, 0.f);
@@ -378,8 +383,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         }
         float sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-        for (uint32_t r = 0; r < kTileMaxCluster; ++r) {
-            const float weight = weight_of(m[r], M);
+        for (uint32_t r = 0; r < kMaxCluster; ++r) {
+            const float weight = partial_weight(m[r], M);
             sum += weight * l[r];
             x += weight * o[r].x;
             y += weight * o[r].y;
@@ -485,10 +490,6 @@ __device__ __forceinline__ uint32_t dim_of(uint32_t lane, int i) {
     return VECT ? lane * EPL + i : lane + 32 * i;
 }
 
-// Weight of a partial result whose maximum is m in one whose maximum is M; a
-// partial result without a score above -inf has none.
-__device__ __forceinline__ float partial_weight(float m, float M) { return m == -INFINITY ? 0.f : exp2f(m - M); }
-
 template <typename T, int EPL, int GH, bool VECT>
 __global__ void __launch_bounds__(kAnyThreads) decode_selected_any(const SelectedParams p) {
     constexpr int TT = EPL == 8 || GH == 8 ? 4 : 8;  // tokens per step (their K and V are in registers)
@@ -499,11 +500,14 @@ __global__ void __launch_bounds__(kAnyThreads) decode_selected_any(const Selecte
     __shared__ float part_o[kAnyWarps][GH][EPL * 32];
     __shared__ float part_m[kAnyWarps][GH], part_l[kAnyWarps][GH];
     __shared__ uint32_t part_seen[kAnyWarps];
+    __shared__ float joined_m[GH], joined_l[GH];
+    __shared__ uint32_t joined_seen;
 
     wait_for_previous_kernel();
     allow_next_kernel();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t seg = blockIdx.x;
+    const uint32_t cluster = p.cluster, rank = blockIdx.x % cluster;
+    const uint32_t seg = blockIdx.x / cluster;
     const uint32_t b = seg / p.hkv, head = seg % p.hkv;
     const uint32_t h0 = blockIdx.y * GH;            // heads [h0, h0 + GH) of the group
     const int ctx = p.ctx[b];
@@ -531,30 +535,37 @@ __global__ void __launch_bounds__(kAnyThreads) decode_selected_any(const Selecte
         for (int i = 0; i < EPL; ++i) q[g][i] *= p.scale_log2;
     }
 
+    // The warps of the cluster take p.round listed slots at a time, a lane
+    // finds the address of one slot's K row (null: not attended), a round ahead
+    // of its use.
     const uint64_t slots = ctx > 0 ? static_cast<uint64_t>(p.keep) * p.T : 0;
-    for (uint64_t s0 = static_cast<uint64_t>(warp) * 32; s0 < slots; s0 += kAnyWarps * 32) {
-        // this lane's slot: the address of its K row, or null
-        const T* mine = nullptr;
-        const uint64_t slot = s0 + lane;
-        if (slot < slots) {
-            const int32_t blk = list[slot / p.T];
-            const uint32_t tok = static_cast<uint32_t>(slot % p.T);
-            if (blk >= 0) {
-                if (static_cast<uint32_t>(blk) >= nblk) {
-                    record_error(p.err, kErrBadBlockId);
-                } else if (static_cast<uint32_t>(blk) * p.T + tok < static_cast<uint32_t>(ctx)) {
-                    const int32_t id = table[blk];
-                    if (static_cast<uint32_t>(id) >= p.num_blocks)
-                        record_error(p.err, kErrBadBlockId);
-                    else
-                        mine = reinterpret_cast<const T*>(p.pool + static_cast<size_t>(id) * p.block_stride) +
-                               static_cast<size_t>(p.layer) * 2 * p.T * row + tok * row + static_cast<size_t>(head) * p.D;
-                }
-            }
+    const uint64_t stride = static_cast<uint64_t>(cluster) * kAnyWarps * p.round;
+    auto row_of = [&](uint64_t slot) -> const T* {
+        if (lane >= p.round || slot >= slots) return nullptr;
+        const int32_t blk = list[slot / p.T];
+        const uint32_t tok = static_cast<uint32_t>(slot % p.T);
+        if (blk < 0) return nullptr;
+        if (static_cast<uint32_t>(blk) >= nblk) {
+            record_error(p.err, kErrBadBlockId);
+            return nullptr;
         }
+        if (static_cast<uint32_t>(blk) * p.T + tok >= static_cast<uint32_t>(ctx)) return nullptr;
+        const int32_t id = table[blk];
+        if (static_cast<uint32_t>(id) >= p.num_blocks) {
+            record_error(p.err, kErrBadBlockId);
+            return nullptr;
+        }
+        return reinterpret_cast<const T*>(p.pool + static_cast<size_t>(id) * p.block_stride) +
+               static_cast<size_t>(p.layer) * 2 * p.T * row + tok * row + static_cast<size_t>(head) * p.D;
+    };
+    uint64_t s0 = static_cast<uint64_t>(rank * kAnyWarps + warp) * p.round;
+    const T* next = row_of(s0 + lane);
+    for (; s0 < slots; s0 += stride) {
+        const T* mine = next;
+        next = row_of(s0 + stride + lane);
         const uint32_t valid = __ballot_sync(0xffffffffu, mine != nullptr);
         seen += __popc(valid);
-        for (uint32_t t0 = 0; t0 < 32; t0 += TT) {
+        for (uint32_t t0 = 0; t0 < p.round; t0 += TT) {
             if (((valid >> t0) & ((1ull << TT) - 1)) == 0) continue;
             float k[TT][EPL], v[TT][EPL];
 #pragma unroll
@@ -626,10 +637,15 @@ __global__ void __launch_bounds__(kAnyThreads) decode_selected_any(const Selecte
     __syncthreads();
     uint32_t any = 0;
 #pragma unroll
-    for (int w = 0; w < kAnyWarps; ++w) any += part_seen[w];
-    for (uint32_t i = threadIdx.x; i < GH * p.D; i += kAnyThreads) {
+    for (int w = 0; w < kAnyWarps; ++w) any |= part_seen[w];
+    auto write_out = [&](uint32_t g, uint32_t d, float acc, float sum) {
+        const size_t h = static_cast<size_t>(head) * p.group + h0 + g;
+        static_cast<T*>(p.out)[(static_cast<size_t>(b) * p.hq + h) * p.D + d] =
+            from_float<T>(any == 0 ? 0.f : acc / sum);
+    };
+    const uint32_t heads = min(static_cast<uint32_t>(GH), p.group - h0);
+    for (uint32_t i = threadIdx.x; i < heads * p.D; i += kAnyThreads) {
         const uint32_t g = i / p.D, d = i % p.D;
-        if (h0 + g >= p.group) break;
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kAnyWarps; ++w) M = fmaxf(M, part_m[w][g]);
@@ -637,24 +653,59 @@ __global__ void __launch_bounds__(kAnyThreads) decode_selected_any(const Selecte
 #pragma unroll
         for (int w = 0; w < kAnyWarps; ++w) {
             const float c = partial_weight(part_m[w][g], M);
-            // a NaN score leaves the maximum at -inf but not the sum
-            sum += part_m[w][g] == -INFINITY ? part_l[w][g] : c * part_l[w][g];
-            acc += part_m[w][g] == -INFINITY ? part_o[w][g][d] : c * part_o[w][g][d];
+            sum += c * part_l[w][g];
+            acc += c * part_o[w][g][d];
         }
-        const size_t h = static_cast<size_t>(head) * p.group + h0 + g;
-        static_cast<T*>(p.out)[(static_cast<size_t>(b) * p.hq + h) * p.D + d] =
-            from_float<T>(any == 0 ? 0.f : acc / sum);
+        if (cluster == 1) {
+            write_out(g, d, acc, sum);
+        } else {
+            part_o[0][g][d] = acc;
+            if (d == 0) {
+                joined_m[g] = M;
+                joined_l[g] = sum;
+                joined_seen = any;
+            }
+        }
     }
+    if (cluster == 1) return;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    for (uint32_t i = rank * kAnyThreads + threadIdx.x; i < heads * p.D; i += cluster * kAnyThreads) {
+        const uint32_t g = i / p.D, d = i % p.D;
+        float m[kMaxCluster], l[kMaxCluster], o[kMaxCluster], M = -INFINITY;
+#pragma unroll
+        for (uint32_t r = 0; r < kMaxCluster; ++r) {
+            m[r] = -INFINITY;
+            l[r] = o[r] = 0.f;
+            if (r < cluster) {
+                m[r] = *cl.map_shared_rank(&joined_m[g], r);
+                l[r] = *cl.map_shared_rank(&joined_l[g], r);
+                o[r] = *cl.map_shared_rank(&part_o[0][g][d], r);
+                any |= *cl.map_shared_rank(&joined_seen, r);
+            }
+            M = fmaxf(M, m[r]);
+        }
+        float sum = 0.f, acc = 0.f;
+#pragma unroll
+        for (uint32_t r = 0; r < kMaxCluster; ++r) {
+            const float c = partial_weight(m[r], M);
+            sum += c * l[r];
+            acc += c * o[r];
+        }
+        write_out(g, d, acc, sum);
+    }
+    // no CTA leaves while another may read its shared memory
+    cl.sync();
 }
 
 template <typename T, int EPL, int GH>
 int launch_any_t(const SelectedParams& p, bool vect, uint32_t segments, cudaStream_t st) {
-    const dim3 grid(segments, ceil_div(p.group, GH));
+    const dim3 grid(segments * p.cluster, ceil_div(p.group, GH));
     if (vect)
         return launch_dependent("launch decode_selected", decode_selected_any<T, EPL, GH, true>, grid, kAnyThreads, 0,
-                                1, st, p);
-    return launch_dependent("launch decode_selected", decode_selected_any<T, EPL, GH, false>, grid, kAnyThreads, 0, 1,
-                            st, p);
+                                p.cluster, st, p);
+    return launch_dependent("launch decode_selected", decode_selected_any<T, EPL, GH, false>, grid, kAnyThreads, 0,
+                            p.cluster, st, p);
 }
 
 template <typename T, int EPL>
@@ -746,12 +797,16 @@ extern "C" int qvp_decode_selected(const qvp_decode_selected_args* args, qvp_str
         const uint64_t pieces = static_cast<uint64_t>(p.keep) * (p.T / 16);
         p.cluster = 1;
         // two CTAs are resident per SM: split a list while the whole grid still is
-        while (p.cluster < kTileMaxCluster && segments * p.cluster * 2 <= 2 * sms && pieces > kTileWarps * p.cluster)
+        while (p.cluster < kMaxCluster && segments * p.cluster * 2 <= 2 * sms && pieces > kTileWarps * p.cluster)
             p.cluster *= 2;
         return p.D == 128 ? launch_tile<128, 3>(p, a, static_cast<uint32_t>(segments), st)
                           : launch_tile<64, 6>(p, a, static_cast<uint32_t>(segments), st);
     }
+    const uint64_t slots = static_cast<uint64_t>(p.keep) * p.T;
     p.cluster = 1;
+    while (p.cluster < kMaxCluster && segments * p.cluster * 2 <= 2 * sms && slots > 8 * kAnyWarps * p.cluster)
+        p.cluster *= 2;
+    p.round = slots >= 64ull * kAnyWarps * p.cluster ? 32 : slots >= 32ull * kAnyWarps * p.cluster ? 16 : 8;
     return a.dtype == QVP_DTYPE_F32 ? launch_any<float>(p, a, static_cast<uint32_t>(segments), st)
                                     : launch_any<__nv_bfloat16>(p, a, static_cast<uint32_t>(segments), st);
 }
