@@ -48,7 +48,7 @@ struct SelectedParams {
 };
 
 // ---------------------------------------------------------------------------
-// bf16, head_dim 64 or 128, blocks of a multiple of 16 tokens, unpadded.
+// bf16, head_dim 64, 96 or 128, blocks of 8 or a multiple of 16 tokens, unpadded.
 //
 // The work of a (sequence, kv head) is a list of 16-token pieces, dealt round
 // robin to the warps of a cluster of CTAs. Each warp streams its own pieces
@@ -70,38 +70,63 @@ struct SelectedParams {
 constexpr int kTileWarps = 4;
 constexpr int kTileThreads = kTileWarps * 32;
 
+// How a piece's 16 tokens lie in the pool: one block (K and V adjacent, one
+// copy), part of a longer block (a copy each), or two blocks of 8 (a copy per
+// block).
+enum PieceKind { kWhole, kPart, kTwo };
+
+// A piece in shared memory: rows of HALF elements, swizzled, as the copies
+// leave them.
+template <int D, PieceKind KIND>
+struct PieceLayout {
+    static constexpr int kHalf = D % 64 == 0 ? 64 : 32;               // elements of a row
+    static constexpr uint32_t kRow = kHalf * 2;                       // bytes of a row
+    static constexpr uint32_t kBoxRows = KIND == kWhole ? 32 : 16;    // rows of one copy's box, per half
+    static constexpr uint32_t kDh = kBoxRows * kRow;                  // between halves of head_dim
+    static constexpr uint32_t kUpper = KIND == kTwo ? 16 * D * 2 : 8 * kRow;                    // to tokens 8 .. 15
+    static constexpr uint32_t kV = KIND == kWhole ? 16 * kRow : KIND == kPart ? 16 * D * 2 : 8 * kRow;  // K to V
+
+    // 16-byte chunk `chunk` (of head_dim) of K token `upper * 8 + row`
+    static __device__ __forceinline__ uint32_t at(uint32_t piece, int chunk, int upper, int row) {
+        constexpr int kChunks = kHalf / 8;
+        const int swizzle = kHalf == 64 ? row : row >> 1;
+        return piece + static_cast<uint32_t>(chunk / kChunks) * kDh + static_cast<uint32_t>(upper) * kUpper +
+               static_cast<uint32_t>(row) * kRow + static_cast<uint32_t>(((chunk % kChunks) ^ swizzle) << 4);
+    }
+};
+
 template <int D, int STAGES>
 struct TileShape {
-    static constexpr uint32_t kPiece = 2 * 16 * D * 2;               // K and V of 16 tokens of one head
+    static constexpr uint32_t kPiece = 2 * 16 * D * 2;
     static constexpr uint32_t kRing = STAGES * kPiece;               // one warp's
     static constexpr uint32_t kBars = kTileWarps * kRing;            // offset of the barriers
     static constexpr uint32_t kStats = kBars + kTileWarps * STAGES * 8;  // m, l of 16 rows per warp, tokens seen
     static constexpr uint32_t kJoined = kStats + kTileWarps * (32 * 4 + 16);  // the same of the whole CTA
     static constexpr uint32_t kSmem = kJoined + 32 * 4 + 16 + 1024;
     static_assert(kRing >= 16 * D * 4, "a warp's partial output takes the place of its ring");
+    static_assert(kPiece % 1024 == 0 && STAGES <= 8, "pieces start on swizzle boundaries, their counts fit 64 bits");
 };
 
-// One piece: online-softmax update of the 16 rows of `st`. `valid` of its
-// tokens are below the context. Where PAIR, rows 8..15 carry the remainders
-// of the weights of rows 0..7 (st.m1, st.l1 unused).
-template <int D, bool PAIR, bool SPLIT>
-__device__ __forceinline__ void attend_piece(WarpState<D>& st, const uint32_t (&qa)[D / 16][4], uint32_t piece,
-                                             int valid, float scale_log2, int lane) {
-    // K and V of a 64-column half: K | V adjacent in one box, or all K before all V
-    constexpr uint32_t kHalf = SPLIT ? 2048u : 4096u;
-    constexpr uint32_t kV = SPLIT ? static_cast<uint32_t>(D / 64) * 2048u : 2048u;
+// One piece: online-softmax update of the 16 rows of `st`. The first va of its
+// tokens 0 .. 7 and the first vb of its tokens 8 .. 15 are attended. Where
+// PAIR, rows 8..15 carry the remainders of the weights of rows 0..7 (st.m1,
+// st.l1 unused).
+template <int D, bool PAIR, PieceKind KIND>
+__device__ __forceinline__ void attend_piece(WarpState<D>& st, const uint32_t (&qa)[D / 16][4], uint32_t piece, int va,
+                                             int vb, float scale_log2, int lane) {
+    using L = PieceLayout<D, KIND>;
     const int c = lane & 3;
     const int mi = lane >> 3;
     const int li = lane & 7;
     float s[2][4];
 #pragma unroll
     for (int a = 0; a < 2; ++a) s[a][0] = s[a][1] = s[a][2] = s[a][3] = 0.f;
+    // the lane's row and swizzle are the same in every step: at(chunk) differs
+    // by a constant and the chunk's bits
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-        const int chunk = ((ks & 3) << 1) + (mi & 1);
-        const int t = ((mi >> 1) << 3) + li;
         uint32_t r0, r1, r2, r3;
-        ldmatrix_x4(box_addr(piece + (ks >> 2) * kHalf, 0, t, chunk), r0, r1, r2, r3);
+        ldmatrix_x4(L::at(piece, 2 * ks + (mi & 1), mi >> 1, li), r0, r1, r2, r3);
         mma_bf16_16816(s[0], qa[ks], r0, r1);
         mma_bf16_16816(s[1], qa[ks], r2, r3);
     }
@@ -114,8 +139,8 @@ __device__ __forceinline__ void attend_piece(WarpState<D>& st, const uint32_t (&
         float x[4];  // this lane's four scores of row g + 8 r: keys 2c, 2c + 1, 8 + 2c, 9 + 2c
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int tok = (e >> 1) * 8 + c * 2 + (e & 1);
-            x[e] = tok < valid ? s[e >> 1][2 * r + (e & 1)] * scale_log2 : -INFINITY;
+            const bool seen = c * 2 + (e & 1) < (e < 2 ? va : vb);
+            x[e] = seen ? s[e >> 1][2 * r + (e & 1)] * scale_log2 : -INFINITY;
         }
         float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -153,15 +178,13 @@ __device__ __forceinline__ void attend_piece(WarpState<D>& st, const uint32_t (&
     }
 #pragma unroll
     for (int np = 0; np < D / 16; ++np) {
-        const int chunk = ((np & 3) << 1) + (mi >> 1);
-        const int t = ((mi & 1) << 3) + li;
         uint32_t v0, v1, v2, v3;
-        ldmatrix_x4_trans(box_addr(piece + (np >> 2) * kHalf + kV, 0, t, chunk), v0, v1, v2, v3);
-        if (valid < 16) {  // V slots past the context may hold anything, NaN included
-            v0 = mask_pair(v0, c * 2, valid);
-            v2 = mask_pair(v2, c * 2, valid);
-            v1 = mask_pair(v1, 8 + c * 2, valid);
-            v3 = mask_pair(v3, 8 + c * 2, valid);
+        ldmatrix_x4_trans(L::at(piece + L::kV, 2 * np + (mi >> 1), mi & 1, li), v0, v1, v2, v3);
+        if (va + vb < 16) {  // V slots that are not attended may hold anything, NaN included
+            v0 = mask_pair(v0, c * 2, va);
+            v2 = mask_pair(v2, c * 2, va);
+            v1 = mask_pair(v1, c * 2, vb);
+            v3 = mask_pair(v3, c * 2, vb);
         }
         mma_bf16_16816(st.o[2 * np], pa, v0, v1);
         mma_bf16_16816(st.o[2 * np + 1], pa, v2, v3);
@@ -169,7 +192,7 @@ __device__ __forceinline__ void attend_piece(WarpState<D>& st, const uint32_t (&
 }
 
 // grid (segments * cluster, chunks of 16 heads of a group)
-template <int D, int STAGES, bool PAIR, bool SPLIT>
+template <int D, int STAGES, bool PAIR, PieceKind KIND>
 __global__ void __launch_bounds__(kTileThreads, 2)
     decode_selected_tile(const __grid_constant__ CUtensorMap tmap, const SelectedParams p) {
     using S = TileShape<D, STAGES>;
@@ -196,14 +219,26 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     const size_t h0 = static_cast<size_t>(head) * p.group + blockIdx.y * 16;
     const int32_t* list = p.selected + static_cast<size_t>(seg) * p.keep;
     const int32_t* table = p.tables + static_cast<size_t>(b) * p.pitch;
-    const uint32_t per_block = p.T / 16;
-    const uint64_t pieces = static_cast<uint64_t>(p.keep) * per_block;
+    constexpr int kBlocks = KIND == kTwo ? 2 : 1;                  // blocks of a piece
+    const uint32_t per_block = KIND == kPart ? p.T / 16 : 1;       // pieces of a block
+    const uint64_t pieces = (static_cast<uint64_t>(p.keep) * per_block + kBlocks - 1) / kBlocks;
     const uint32_t workers = cluster * kTileWarps, worker = rank * kTileWarps + warp;
-    // The lane's piece of a round of 32 per warp: its listed block (-1: none)
-    // and that block's frame. Neither load waits for the context length.
-    auto block_of = [&](uint64_t i) { return i < pieces ? list[i / per_block] : -1; };
-    auto frame_of = [&](int32_t blk) { return static_cast<uint32_t>(blk) < p.pitch ? table[blk] : -1; };
-    int32_t blk = block_of(worker + static_cast<uint64_t>(workers) * lane);
+    // The lane's piece of a window of 32 per warp: its listed blocks (-1:
+    // none) and their frames. Neither load waits for the context length.
+    int32_t blk[kBlocks], frame[kBlocks];
+    auto load_blocks = [&](uint64_t i) {
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+            const uint64_t e = kBlocks * (i / per_block) + k;
+            blk[k] = e < p.keep ? list[e] : -1;
+        }
+    };
+    auto load_frames = [&]() {
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) frame[k] = static_cast<uint32_t>(blk[k]) < p.pitch ? table[blk[k]] : -1;
+    };
+    uint64_t mine = worker + static_cast<uint64_t>(workers) * lane;
+    load_blocks(mine);
     const int ctx = p.ctx[b];
 
     uint32_t qa[D / 16][4];
@@ -221,7 +256,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             qa[ks][3] = g + 8 < G ? q_hi[k0 + 4] : 0u;
         }
     }
-    int32_t frame = frame_of(blk);
+    load_frames();
     if (ctx < 0 || static_cast<uint32_t>(ctx) > p.capacity) {  // the whole cluster
         if (threadIdx.x == 0) record_error(p.err, kErrBadContext);
         return;
@@ -231,58 +266,85 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     st.reset();
     uint32_t seen = 0;                      // tokens attended by this warp
     uint32_t issued = 0, used = 0;          // pieces of this warp
-    bool alive = true;
+    uint64_t counts = 0;                    // va and vb of each slot's piece, 4 bits each
     const uint64_t policy = l2_policy_evict_first();
 
-    for (uint64_t base = worker; alive && base < pieces; base += static_cast<uint64_t>(workers) * 32) {
-        // the piece's K row in the pool and the tokens it has below the
-        // context (0: nothing to attend)
-        const uint64_t i = base + static_cast<uint64_t>(workers) * lane;
-        const uint32_t first = static_cast<uint32_t>(i % per_block) * 16;
-        int valid = 0, krow = 0;
-        if (blk >= 0 && ctx > 0) {
-            if (static_cast<uint32_t>(blk) >= nblk || static_cast<uint32_t>(frame) >= p.num_blocks) {
-                record_error(p.err, kErrBadBlockId);
-            } else {
-                valid = max(0, min(16, ctx - static_cast<int>(static_cast<uint32_t>(blk) * p.T + first)));
-                krow = static_cast<int>(((static_cast<uint32_t>(frame) * p.num_layers + p.layer) * 2) * p.T + first);
+    // the window: K rows of the lane's piece in the pool, the tokens to attend
+    // of its halves, and the lanes whose pieces are still to be copied
+    int krow[kBlocks], va = 0, vb = 0;
+    uint32_t to_issue = 0;
+    uint64_t base = worker;                 // the next window's first piece
+    auto next_window = [&]() {
+        const uint32_t first = KIND == kPart ? static_cast<uint32_t>(mine % per_block) * 16 : 0u;
+        int left[kBlocks];                  // tokens from the piece's first to the context's end
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+            left[k] = 0;
+            krow[k] = 0;
+            if (blk[k] >= 0 && ctx > 0) {
+                if (static_cast<uint32_t>(blk[k]) >= nblk || static_cast<uint32_t>(frame[k]) >= p.num_blocks) {
+                    record_error(p.err, kErrBadBlockId);
+                } else {
+                    left[k] = ctx - static_cast<int>(static_cast<uint32_t>(blk[k]) * p.T + first);
+                    krow[k] = static_cast<int>(((static_cast<uint32_t>(frame[k]) * p.num_layers + p.layer) * 2) * p.T +
+                                               first);
+                }
             }
         }
-        blk = block_of(i + static_cast<uint64_t>(workers) * 32);  // of the next round
-        frame = frame_of(blk);
-        uint32_t to_issue = __ballot_sync(0xffffffffu, valid > 0), to_use = to_issue;
-        auto issue = [&]() {
+        va = max(0, min(8, left[0]));
+        vb = max(0, min(8, KIND == kTwo ? left[kBlocks - 1] : left[0] - 8));
+        to_issue = __ballot_sync(0xffffffffu, va + vb > 0);
+        base += static_cast<uint64_t>(workers) * 32;
+        mine += static_cast<uint64_t>(workers) * 32;
+        load_blocks(mine);                  // of the window after it
+        load_frames();
+    };
+    // Copies pieces into the free slots of the ring.
+    auto fill = [&]() {
+        while (issued - used < STAGES) {
+            while (to_issue == 0) {
+                if (base >= pieces) return;
+                next_window();
+            }
             const int from = __ffs(to_issue) - 1;
             to_issue &= to_issue - 1;
-            const int row = __shfl_sync(0xffffffffu, krow, from);
+            const uint32_t slot = issued % STAGES;
+            const uint32_t na = __shfl_sync(0xffffffffu, va, from), nb = __shfl_sync(0xffffffffu, vb, from);
+            int row[kBlocks];
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k) row[k] = __shfl_sync(0xffffffffu, krow[k], from);
+            counts = (counts & ~(0xffull << (8 * slot))) | (static_cast<uint64_t>(na | nb << 4) << (8 * slot));
             if (lane == 0) {
-                const uint32_t slot = issued % STAGES;
                 const uint32_t dst = ring + slot * S::kPiece, bar = bars + 8 * slot;
-                mbar_arrive_expect_tx(bar, S::kPiece);
-                tma_load_4d(dst, &tmap, bar, 0, row, static_cast<int>(head), 0, policy);
-                if constexpr (SPLIT)
-                    tma_load_4d(dst + S::kPiece / 2, &tmap, bar, 0, row + static_cast<int>(p.T), static_cast<int>(head),
-                                0, policy);
+                const int h = static_cast<int>(head);
+                if constexpr (KIND == kTwo) {
+                    mbar_arrive_expect_tx(bar, (na > 0) == (nb > 0) ? S::kPiece : S::kPiece / 2);
+                    if (na > 0) tma_load_4d(dst, &tmap, bar, 0, row[0], h, 0, policy);
+                    if (nb > 0) tma_load_4d(dst + S::kPiece / 2, &tmap, bar, 0, row[kBlocks - 1], h, 0, policy);
+                } else {
+                    mbar_arrive_expect_tx(bar, S::kPiece);
+                    tma_load_4d(dst, &tmap, bar, 0, row[0], h, 0, policy);
+                    if constexpr (KIND == kPart)
+                        tma_load_4d(dst + S::kPiece / 2, &tmap, bar, 0, row[0] + static_cast<int>(p.T), h, 0, policy);
+                }
             }
             ++issued;
-        };
-        while (to_issue != 0 && issued - used < STAGES) issue();
-        while (to_use != 0) {
-            const int from = __ffs(to_use) - 1;
-            to_use &= to_use - 1;
-            const int n = __shfl_sync(0xffffffffu, valid, from);
-            const uint32_t slot = used % STAGES;
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * slot, (used / STAGES) & 1u))) {
-                if (lane == 0) record_error(p.err, kErrWaitTimeout);
-                alive = false;
-                break;
-            }
-            attend_piece<D, PAIR, SPLIT>(st, qa, ring + slot * S::kPiece, n, p.scale_log2, lane);
-            seen += n;
-            ++used;
-            __syncwarp();  // every lane has read the slot before it is filled again
-            if (to_issue != 0) issue();
         }
+    };
+    fill();
+    while (used < issued) {
+        const uint32_t slot = used % STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * slot, (used / STAGES) & 1u))) {
+            if (lane == 0) record_error(p.err, kErrWaitTimeout);
+            break;
+        }
+        const uint32_t n = static_cast<uint32_t>(counts >> (8 * slot));
+        const int na = n & 15, nb = (n >> 4) & 15;
+        attend_piece<D, PAIR, KIND>(st, qa, ring + slot * S::kPiece, na, nb, p.scale_log2, lane);
+        seen += na + nb;
+        ++used;
+        __syncwarp();  // every lane has read the slot before it is filled again
+        fill();
     }
     // after a wait that ran out, no copy may still be landing below
     for (; used < issued; ++used) mbar_wait_bounded(bars + 8 * (used % STAGES), (used / STAGES) & 1u);
@@ -395,29 +457,33 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     cl.sync();
 }
 
-template <int D, int STAGES, bool PAIR, bool SPLIT>
+template <int D, int STAGES, bool PAIR, PieceKind KIND>
 int launch_tile_t(const SelectedParams& p, const qvp_decode_selected_args& a, uint32_t segments, cudaStream_t st) {
     using S = TileShape<D, STAGES>;
+    using L = PieceLayout<D, KIND>;
     static std::atomic<std::uint64_t> attr_done{0};
-    auto kern = decode_selected_tile<D, STAGES, PAIR, SPLIT>;
+    auto kern = decode_selected_tile<D, STAGES, PAIR, KIND>;
     int rc = set_smem_limit_once(attr_done, reinterpret_cast<const void*>(kern), S::kSmem,
                                  "cudaFuncSetAttribute(decode_selected)");
     if (rc != QVP_OK) return rc;
     CUtensorMap map;
-    rc = make_pool_map(a.pool, a.num_blocks, a.shape, 1, SPLIT ? 16 : 32, D / 64, &map);
+    rc = make_pool_map(a.pool, a.num_blocks, a.shape, 1, L::kBoxRows, D / L::kHalf, &map, L::kHalf);
     if (rc != QVP_OK) return rc;
     const dim3 grid(segments * p.cluster, ceil_div(p.group, 16));
     return launch_dependent("launch decode_selected", kern, grid, kTileThreads, S::kSmem, p.cluster, st, map, p);
 }
 
+template <int D, int STAGES, bool PAIR>
+int launch_tile_k(const SelectedParams& p, const qvp_decode_selected_args& a, uint32_t segments, cudaStream_t st) {
+    if (p.T == 16) return launch_tile_t<D, STAGES, PAIR, kWhole>(p, a, segments, st);
+    if (p.T == 8) return launch_tile_t<D, STAGES, PAIR, kTwo>(p, a, segments, st);
+    return launch_tile_t<D, STAGES, PAIR, kPart>(p, a, segments, st);
+}
+
 template <int D, int STAGES>
 int launch_tile(const SelectedParams& p, const qvp_decode_selected_args& a, uint32_t segments, cudaStream_t st) {
-    const bool split = p.T != 16;
-    if (p.group <= 8)
-        return split ? launch_tile_t<D, STAGES, true, true>(p, a, segments, st)
-                     : launch_tile_t<D, STAGES, true, false>(p, a, segments, st);
-    return split ? launch_tile_t<D, STAGES, false, true>(p, a, segments, st)
-                 : launch_tile_t<D, STAGES, false, false>(p, a, segments, st);
+    return p.group <= 8 ? launch_tile_k<D, STAGES, true>(p, a, segments, st)
+                        : launch_tile_k<D, STAGES, false>(p, a, segments, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -789,18 +855,21 @@ extern "C" int qvp_decode_selected(const qvp_decode_selected_args* args, qvp_str
     p.scale_log2 = a.scale * 1.4426950408889634f;  // log2(e)
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const uint64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
-    const bool tile = a.dtype == QVP_DTYPE_BF16 && (p.D == 64 || p.D == 128) && p.T % 16 == 0 &&
+    const bool tile = a.dtype == QVP_DTYPE_BF16 && (p.D == 64 || p.D == 96 || p.D == 128) &&
+                      (p.T % 16 == 0 || p.T == 8) &&
                       a.block_stride == qvp_block_bytes(&sh) && aligned_to(a.pool, 16) && aligned_to(a.query, 4) &&
                       q_pitch % 2 == 0 && aligned_to(a.out, 4) &&
                       static_cast<uint64_t>(a.num_blocks) * sh.num_layers * 2 * p.T < (1ull << 31);
     if (tile) {
-        const uint64_t pieces = static_cast<uint64_t>(p.keep) * (p.T / 16);
+        const uint64_t pieces = (static_cast<uint64_t>(p.keep) * p.T + 15) / 16;
         p.cluster = 1;
         // two CTAs are resident per SM: split a list while the whole grid still is
         while (p.cluster < kMaxCluster && segments * p.cluster * 2 <= 2 * sms && pieces > kTileWarps * p.cluster)
             p.cluster *= 2;
-        return p.D == 128 ? launch_tile<128, 3>(p, a, static_cast<uint32_t>(segments), st)
-                          : launch_tile<64, 6>(p, a, static_cast<uint32_t>(segments), st);
+        // 24 KiB of copies in flight per warp
+        return p.D == 128  ? launch_tile<128, 3>(p, a, static_cast<uint32_t>(segments), st)
+               : p.D == 96 ? launch_tile<96, 4>(p, a, static_cast<uint32_t>(segments), st)
+                           : launch_tile<64, 6>(p, a, static_cast<uint32_t>(segments), st);
     }
     const uint64_t slots = static_cast<uint64_t>(p.keep) * p.T;
     p.cluster = 1;
