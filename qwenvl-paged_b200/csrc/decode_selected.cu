@@ -48,23 +48,29 @@ struct SelectedParams {
 };
 
 // ---------------------------------------------------------------------------
-// bf16, head_dim 64, 96 or 128, blocks of 8 or a multiple of 16 tokens, unpadded.
+// On the tensor cores: bf16, head_dim 64, 96 or 128, blocks of 8 or a multiple
+// of 16 tokens, unpadded.
 //
 // The work of a (sequence, kv head) is a list of 16-token pieces, dealt round
 // robin to the warps of a cluster of CTAs. Each warp streams its own pieces
-// with TMA into a ring of its own (K and V of a piece: 4 * head_dim * 16
-// bytes) and needs no other warp until the end, so there is no producer warp
-// and no barrier in the loop. Q K^T and P V run on mma.sync m16n8k16 with the
-// group padded to 16 rows; they are a small part of the time (the kernel is
-// bound by HBM), and tcgen05's 128-row tiles would be 6 % full.
+// with TMA into a ring of its own and needs no other warp until the end, so
+// there is no producer warp and no barrier in the loop. Q K^T and P V run on
+// mma.sync with the group padded to 16 rows; they are a small part of the time
+// (the kernel is bound by HBM), and tcgen05's 128-row tiles would be 6 % full.
 //
 // A group of at most 8 heads leaves the upper 8 rows of the tile free: the
-// weights' rounding remainders go there (P = hi + lo, both bf16), so P V
+// remainders of its rounded weights go there (P = hi + lo, both bf16), so P V
 // loses 2^-16 of a weight instead of 2^-8 at no cost. Larger groups multiply
-// bf16 weights, as the dense decode does.
+// bf16 weights, as the dense decode does. An infinity of V does not survive
+// that (inf * hi + inf * lo may be inf - inf): a warp whose sums hold a NaN at
+// the end goes through its pieces again with hi alone, and what is NaN then is
+// NaN.
 //
 // At the end the warps' partial results are joined through distributed shared
 // memory: no workspace, no second kernel, and a fixed order.
+//
+// fp32 is not here: mma.sync on tf32 pairs has the rate of fused multiply-adds
+// on this chip, and took longer than the kernel below.
 // ---------------------------------------------------------------------------
 
 constexpr int kTileWarps = 4;
@@ -95,25 +101,27 @@ struct PieceLayout {
     }
 };
 
-template <int D, int STAGES>
+// Shared memory of a kernel over tiles of kind `Tile`.
+template <typename Tile>
 struct TileShape {
-    static constexpr uint32_t kPiece = 2 * 16 * D * 2;
-    static constexpr uint32_t kRing = STAGES * kPiece;               // one warp's
+    static constexpr int kStages = Tile::kStages;
+    static constexpr uint32_t kPiece = Tile::kPiece;
+    static constexpr uint32_t kRing = kStages * kPiece;              // one warp's
     static constexpr uint32_t kBars = kTileWarps * kRing;            // offset of the barriers
-    static constexpr uint32_t kStats = kBars + kTileWarps * STAGES * 8;  // m, l of 16 rows per warp, tokens seen
+    static constexpr uint32_t kStats = kBars + kTileWarps * kStages * 8;  // m, l of 16 rows per warp, tokens seen
     static constexpr uint32_t kJoined = kStats + kTileWarps * (32 * 4 + 16);  // the same of the whole CTA
     static constexpr uint32_t kSmem = kJoined + 32 * 4 + 16 + 1024;
-    static_assert(kRing >= 16 * D * 4, "a warp's partial output takes the place of its ring");
-    static_assert(kPiece % 1024 == 0 && STAGES <= 8, "pieces start on swizzle boundaries, their counts fit 64 bits");
+    static_assert(kRing >= Tile::kHeads * Tile::kDim * 4, "a warp's partial output takes the place of its ring");
+    static_assert(kPiece % 1024 == 0 && kStages <= 8, "pieces start on swizzle boundaries, their counts fit 64 bits");
 };
 
 // One piece: online-softmax update of the 16 rows of `st`. The first va of its
 // tokens 0 .. 7 and the first vb of its tokens 8 .. 15 are attended. Where
 // PAIR, rows 8..15 carry the remainders of the weights of rows 0..7 (st.m1,
-// st.l1 unused).
+// st.l1 unused), unless `careful`.
 template <int D, bool PAIR, PieceKind KIND>
 __device__ __forceinline__ void attend_piece(WarpState<D>& st, const uint32_t (&qa)[D / 16][4], uint32_t piece, int va,
-                                             int vb, float scale_log2, int lane) {
+                                             int vb, float scale_log2, bool careful, int lane) {
     using L = PieceLayout<D, KIND>;
     const int c = lane & 3;
     const int mi = lane >> 3;
@@ -162,8 +170,8 @@ __device__ __forceinline__ void attend_piece(WarpState<D>& st, const uint32_t (&
                 const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&hi);
                 return pack_bf16x2(u - __low2float(h), w - __high2float(h));
             };
-            pa[1] = low(x[0], x[1], pa[0]);
-            pa[3] = low(x[2], x[3], pa[2]);
+            pa[1] = careful ? 0u : low(x[0], x[1], pa[0]);
+            pa[3] = careful ? 0u : low(x[2], x[3], pa[2]);
         }
     }
     if (__any_sync(0xffffffffu, grew)) {
@@ -191,12 +199,101 @@ __device__ __forceinline__ void attend_piece(WarpState<D>& st, const uint32_t (&
     }
 }
 
-// grid (segments * cluster, chunks of 16 heads of a group)
-template <int D, int STAGES, bool PAIR, PieceKind KIND>
+template <int D, bool PAIR, PieceKind KIND>
+struct Bf16Tile {
+    using T = __nv_bfloat16;
+    static constexpr int kDim = D;
+    static constexpr int kHeads = 16;                                 // of a group at a time
+    static constexpr int kBlocks = KIND == kTwo ? 2 : 1;              // blocks of a piece
+    static constexpr uint32_t kPiece = 2 * 16 * D * 2;                // K and V of its tokens, one head
+    static constexpr int kStages = 24576 / kPiece;                    // 24 KiB of copies in flight per warp
+    static constexpr uint32_t kBoxRows = PieceLayout<D, KIND>::kBoxRows;
+    static constexpr int kHalf = PieceLayout<D, KIND>::kHalf;
+
+    static constexpr bool kSplits = PAIR;
+
+    uint32_t qa[D / 16][4];
+    WarpState<D> st;
+
+    __device__ __forceinline__ void start(const T* q, int G, int lane) {
+        const int g = lane >> 2, c = lane & 3;
+        const uint32_t* q_lo = reinterpret_cast<const uint32_t*>(q + g * D);
+        const uint32_t* q_hi = reinterpret_cast<const uint32_t*>(q + (g + 8) * D);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            const int k0 = (ks * 16 + c * 2) >> 1;
+            qa[ks][0] = g < G ? q_lo[k0] : 0u;
+            qa[ks][1] = g + 8 < G ? q_hi[k0] : 0u;
+            qa[ks][2] = g < G ? q_lo[k0 + 4] : 0u;
+            qa[ks][3] = g + 8 < G ? q_hi[k0 + 4] : 0u;
+        }
+        st.reset();
+    }
+    // Copies the piece whose K rows in the pool are `row` (of each block) to
+    // `dst`; T tokens per block, the first na and nb of its halves attended.
+    static __device__ __forceinline__ void copy(uint32_t dst, const CUtensorMap& tmap, uint32_t bar,
+                                                const int (&row)[kBlocks], int tokens, int head, uint32_t na,
+                                                uint32_t nb, uint64_t policy) {
+        if constexpr (KIND == kTwo) {
+            mbar_arrive_expect_tx(bar, (na > 0) == (nb > 0) ? kPiece : kPiece / 2);
+            if (na > 0) tma_load_4d(dst, &tmap, bar, 0, row[0], head, 0, policy);
+            if (nb > 0) tma_load_4d(dst + kPiece / 2, &tmap, bar, 0, row[kBlocks - 1], head, 0, policy);
+        } else {
+            mbar_arrive_expect_tx(bar, kPiece);
+            tma_load_4d(dst, &tmap, bar, 0, row[0], head, 0, policy);
+            if constexpr (KIND == kPart) tma_load_4d(dst + kPiece / 2, &tmap, bar, 0, row[0] + tokens, head, 0, policy);
+        }
+    }
+    __device__ __forceinline__ void attend(const uint8_t* piece, int na, int nb, float scale_log2, bool careful,
+                                           int lane) {
+        attend_piece<D, PAIR, KIND>(st, qa, smem_u32(piece), na, nb, scale_log2, careful, lane);
+    }
+    __device__ __forceinline__ bool spoiled() const {
+        bool nan = false;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) nan |= isnan(st.o[n][e] + st.o[n][2 + e]);
+        return nan;
+    }
+    __device__ __forceinline__ void restart() { st.reset(); }
+    // This warp's sums: rows of D floats to `part`, maxima and weights' sums to stat.
+    __device__ __forceinline__ void finish(float* part, float* stat, bool careful, int lane) {
+        const int g = lane >> 2, c = lane & 3;
+        st.l0 += __shfl_xor_sync(0xffffffffu, st.l0, 1);
+        st.l0 += __shfl_xor_sync(0xffffffffu, st.l0, 2);
+        st.l1 += __shfl_xor_sync(0xffffffffu, st.l1, 1);
+        st.l1 += __shfl_xor_sync(0xffffffffu, st.l1, 2);
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+            const int col = n * 8 + c * 2;
+            if constexpr (PAIR) {
+                *reinterpret_cast<float2*>(part + g * D + col) =
+                    careful ? make_float2(st.o[n][0], st.o[n][1])
+                            : make_float2(st.o[n][0] + st.o[n][2], st.o[n][1] + st.o[n][3]);
+            } else {
+                *reinterpret_cast<float2*>(part + g * D + col) = make_float2(st.o[n][0], st.o[n][1]);
+                *reinterpret_cast<float2*>(part + (g + 8) * D + col) = make_float2(st.o[n][2], st.o[n][3]);
+            }
+        }
+        if (c == 0) {
+            stat[g] = st.m0;
+            stat[16 + g] = st.l0;
+            if constexpr (!PAIR) {
+                stat[8 + g] = st.m1;
+                stat[24 + g] = st.l1;
+            }
+        }
+    }
+};
+
+// grid (segments * cluster, chunks of Tile::kHeads heads of a group)
+template <typename Tile>
 __global__ void __launch_bounds__(kTileThreads, 2)
     decode_selected_tile(const __grid_constant__ CUtensorMap tmap, const SelectedParams p) {
-    using S = TileShape<D, STAGES>;
-    constexpr int NT = D / 8;
+    using S = TileShape<Tile>;
+    using T = __nv_bfloat16;
+    constexpr int D = Tile::kDim, STAGES = Tile::kStages, kBlocks = Tile::kBlocks;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
@@ -215,12 +312,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     const uint32_t cluster = p.cluster;
     const uint32_t rank = blockIdx.x % cluster, seg = blockIdx.x / cluster;
     const uint32_t b = seg / p.hkv, head = seg % p.hkv;
-    const int G = static_cast<int>(min(p.group - blockIdx.y * 16, 16u));  // heads of this chunk
-    const size_t h0 = static_cast<size_t>(head) * p.group + blockIdx.y * 16;
+    const int G = static_cast<int>(min(p.group - blockIdx.y * Tile::kHeads, static_cast<uint32_t>(Tile::kHeads)));
+    const size_t h0 = static_cast<size_t>(head) * p.group + blockIdx.y * Tile::kHeads;
     const int32_t* list = p.selected + static_cast<size_t>(seg) * p.keep;
     const int32_t* table = p.tables + static_cast<size_t>(b) * p.pitch;
-    constexpr int kBlocks = KIND == kTwo ? 2 : 1;                  // blocks of a piece
-    const uint32_t per_block = KIND == kPart ? p.T / 16 : 1;       // pieces of a block
+    const uint32_t per_block = kBlocks == 1 ? p.T / 16 : 1;  // pieces of a block
     const uint64_t pieces = (static_cast<uint64_t>(p.keep) * per_block + kBlocks - 1) / kBlocks;
     const uint32_t workers = cluster * kTileWarps, worker = rank * kTileWarps + warp;
     // The lane's piece of a window of 32 per warp: its listed blocks (-1:
@@ -241,29 +337,14 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     load_blocks(mine);
     const int ctx = p.ctx[b];
 
-    uint32_t qa[D / 16][4];
-    {
-        const int g = lane >> 2, c = lane & 3;
-        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) + b * p.q_pitch + h0 * D;
-        const uint32_t* q_lo = reinterpret_cast<const uint32_t*>(q + g * D);
-        const uint32_t* q_hi = reinterpret_cast<const uint32_t*>(q + (g + 8) * D);
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            const int k0 = (ks * 16 + c * 2) >> 1;
-            qa[ks][0] = g < G ? q_lo[k0] : 0u;
-            qa[ks][1] = g + 8 < G ? q_hi[k0] : 0u;
-            qa[ks][2] = g < G ? q_lo[k0 + 4] : 0u;
-            qa[ks][3] = g + 8 < G ? q_hi[k0 + 4] : 0u;
-        }
-    }
+    Tile tile;
+    tile.start(static_cast<const T*>(p.q) + b * p.q_pitch + h0 * D, G, lane);
     load_frames();
     if (ctx < 0 || static_cast<uint32_t>(ctx) > p.capacity) {  // the whole cluster
         if (threadIdx.x == 0) record_error(p.err, kErrBadContext);
         return;
     }
     const uint32_t nblk = (static_cast<uint32_t>(ctx) + p.T - 1) / p.T;
-    WarpState<D> st;
-    st.reset();
     uint32_t seen = 0;                      // tokens attended by this warp
     uint32_t issued = 0, used = 0;          // pieces of this warp
     uint64_t counts = 0;                    // va and vb of each slot's piece, 4 bits each
@@ -275,7 +356,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     uint32_t to_issue = 0;
     uint64_t base = worker;                 // the next window's first piece
     auto next_window = [&]() {
-        const uint32_t first = KIND == kPart ? static_cast<uint32_t>(mine % per_block) * 16 : 0u;
+        const uint32_t first = static_cast<uint32_t>(mine % per_block) * 16;
         int left[kBlocks];                  // tokens from the piece's first to the context's end
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) {
@@ -292,7 +373,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             }
         }
         va = max(0, min(8, left[0]));
-        vb = max(0, min(8, KIND == kTwo ? left[kBlocks - 1] : left[0] - 8));
+        vb = max(0, min(8, kBlocks == 2 ? left[kBlocks - 1] : left[0] - 8));
         to_issue = __ballot_sync(0xffffffffu, va + vb > 0);
         base += static_cast<uint64_t>(workers) * 32;
         mine += static_cast<uint64_t>(workers) * 32;
@@ -314,78 +395,55 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) row[k] = __shfl_sync(0xffffffffu, krow[k], from);
             counts = (counts & ~(0xffull << (8 * slot))) | (static_cast<uint64_t>(na | nb << 4) << (8 * slot));
-            if (lane == 0) {
-                const uint32_t dst = ring + slot * S::kPiece, bar = bars + 8 * slot;
-                const int h = static_cast<int>(head);
-                if constexpr (KIND == kTwo) {
-                    mbar_arrive_expect_tx(bar, (na > 0) == (nb > 0) ? S::kPiece : S::kPiece / 2);
-                    if (na > 0) tma_load_4d(dst, &tmap, bar, 0, row[0], h, 0, policy);
-                    if (nb > 0) tma_load_4d(dst + S::kPiece / 2, &tmap, bar, 0, row[kBlocks - 1], h, 0, policy);
-                } else {
-                    mbar_arrive_expect_tx(bar, S::kPiece);
-                    tma_load_4d(dst, &tmap, bar, 0, row[0], h, 0, policy);
-                    if constexpr (KIND == kPart)
-                        tma_load_4d(dst + S::kPiece / 2, &tmap, bar, 0, row[0] + static_cast<int>(p.T), h, 0, policy);
-                }
-            }
+            if (lane == 0)
+                Tile::copy(ring + slot * S::kPiece, tmap, bars + 8 * slot, row, static_cast<int>(p.T),
+                           static_cast<int>(head), na, nb, policy);
             ++issued;
         }
     };
-    fill();
-    while (used < issued) {
-        const uint32_t slot = used % STAGES;
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * slot, (used / STAGES) & 1u))) {
-            if (lane == 0) record_error(p.err, kErrWaitTimeout);
-            break;
-        }
-        const uint32_t n = static_cast<uint32_t>(counts >> (8 * slot));
-        const int na = n & 15, nb = (n >> 4) & 15;
-        attend_piece<D, PAIR, KIND>(st, qa, ring + slot * S::kPiece, na, nb, p.scale_log2, lane);
-        seen += na + nb;
-        ++used;
-        __syncwarp();  // every lane has read the slot before it is filled again
+    bool careful = false;
+    for (;;) {
         fill();
+        while (used < issued) {
+            const uint32_t slot = used % STAGES;
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * slot, (used / STAGES) & 1u))) {
+                if (lane == 0) record_error(p.err, kErrWaitTimeout);
+                break;
+            }
+            const uint32_t n = static_cast<uint32_t>(counts >> (8 * slot));
+            const int na = n & 15, nb = (n >> 4) & 15;
+            tile.attend(smem + warp * S::kRing + slot * S::kPiece, na, nb, p.scale_log2, careful, lane);
+            seen += na + nb;
+            ++used;
+            __syncwarp();  // every lane has read the slot before it is filled again
+            fill();
+        }
+        if (!Tile::kSplits || careful || used < issued || !__any_sync(0xffffffffu, tile.spoiled())) break;
+        // once more from the first piece, without splitting
+        careful = true;
+        tile.restart();
+        seen = 0;
+        base = worker;
+        mine = worker + static_cast<uint64_t>(workers) * lane;
+        load_blocks(mine);
+        load_frames();
     }
     // after a wait that ran out, no copy may still be landing below
     for (; used < issued; ++used) mbar_wait_bounded(bars + 8 * (used % STAGES), (used / STAGES) & 1u);
 
-    // This warp's partial result: 16 rows of D floats in its ring, m and l and
-    // the token count behind the rings.
-    st.l0 += __shfl_xor_sync(0xffffffffu, st.l0, 1);
-    st.l0 += __shfl_xor_sync(0xffffffffu, st.l0, 2);
-    st.l1 += __shfl_xor_sync(0xffffffffu, st.l1, 1);
-    st.l1 += __shfl_xor_sync(0xffffffffu, st.l1, 2);
+    // This warp's partial result: rows of D floats in its ring, m and l and the
+    // token count behind the rings.
     __syncwarp();
     {
-        const int g = lane >> 2, c = lane & 3;
-        float* part = reinterpret_cast<float*>(smem + warp * S::kRing);
         float* stat = reinterpret_cast<float*>(smem + S::kStats) + warp * 36;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int col = n * 8 + c * 2;
-            if constexpr (PAIR) {
-                *reinterpret_cast<float2*>(part + g * D + col) =
-                    make_float2(st.o[n][0] + st.o[n][2], st.o[n][1] + st.o[n][3]);
-            } else {
-                *reinterpret_cast<float2*>(part + g * D + col) = make_float2(st.o[n][0], st.o[n][1]);
-                *reinterpret_cast<float2*>(part + (g + 8) * D + col) = make_float2(st.o[n][2], st.o[n][3]);
-            }
-        }
-        if (c == 0) {
-            stat[g] = st.m0;
-            stat[16 + g] = st.l0;
-            if constexpr (!PAIR) {
-                stat[8 + g] = st.m1;
-                stat[24 + g] = st.l1;
-            }
-        }
+        tile.finish(reinterpret_cast<float*>(smem + warp * S::kRing), stat, careful, lane);
         if (lane == 0) reinterpret_cast<uint32_t*>(stat)[32] = seen;
     }
     __syncthreads();
     // Join the warps, two elements a thread: straight to the output, or to the
     // first warp's place for the cluster.
     const float* stats = reinterpret_cast<const float*>(smem + S::kStats);
-    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + (static_cast<size_t>(b) * p.hq + h0) * D;
+    T* out = static_cast<T*>(p.out) + (static_cast<size_t>(b) * p.hq + h0) * D;
     uint32_t any = 0;
 #pragma unroll
     for (int w = 0; w < kTileWarps; ++w) any |= reinterpret_cast<const uint32_t*>(stats)[w * 36 + 32];
@@ -457,41 +515,42 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     cl.sync();
 }
 
-template <int D, int STAGES, bool PAIR, PieceKind KIND>
+template <typename Tile>
 int launch_tile_t(const SelectedParams& p, const qvp_decode_selected_args& a, uint32_t segments, cudaStream_t st) {
-    using S = TileShape<D, STAGES>;
-    using L = PieceLayout<D, KIND>;
+    using S = TileShape<Tile>;
     static std::atomic<std::uint64_t> attr_done{0};
-    auto kern = decode_selected_tile<D, STAGES, PAIR, KIND>;
+    auto kern = decode_selected_tile<Tile>;
     int rc = set_smem_limit_once(attr_done, reinterpret_cast<const void*>(kern), S::kSmem,
                                  "cudaFuncSetAttribute(decode_selected)");
     if (rc != QVP_OK) return rc;
     CUtensorMap map;
-    rc = make_pool_map(a.pool, a.num_blocks, a.shape, 1, L::kBoxRows, D / L::kHalf, &map, L::kHalf);
+    rc = make_pool_map(a.pool, a.num_blocks, a.shape, 1, Tile::kBoxRows, Tile::kDim / Tile::kHalf, &map, Tile::kHalf);
     if (rc != QVP_OK) return rc;
-    const dim3 grid(segments * p.cluster, ceil_div(p.group, 16));
+    const dim3 grid(segments * p.cluster, ceil_div(p.group, Tile::kHeads));
     return launch_dependent("launch decode_selected", kern, grid, kTileThreads, S::kSmem, p.cluster, st, map, p);
 }
 
-template <int D, int STAGES, bool PAIR>
-int launch_tile_k(const SelectedParams& p, const qvp_decode_selected_args& a, uint32_t segments, cudaStream_t st) {
-    if (p.T == 16) return launch_tile_t<D, STAGES, PAIR, kWhole>(p, a, segments, st);
-    if (p.T == 8) return launch_tile_t<D, STAGES, PAIR, kTwo>(p, a, segments, st);
-    return launch_tile_t<D, STAGES, PAIR, kPart>(p, a, segments, st);
+template <int D, bool PAIR>
+int launch_bf16(const SelectedParams& p, const qvp_decode_selected_args& a, uint32_t segments, cudaStream_t st) {
+    if (p.T == 16) return launch_tile_t<Bf16Tile<D, PAIR, kWhole>>(p, a, segments, st);
+    if (p.T == 8) return launch_tile_t<Bf16Tile<D, PAIR, kTwo>>(p, a, segments, st);
+    return launch_tile_t<Bf16Tile<D, PAIR, kPart>>(p, a, segments, st);
 }
 
-template <int D, int STAGES>
+template <int D>
 int launch_tile(const SelectedParams& p, const qvp_decode_selected_args& a, uint32_t segments, cudaStream_t st) {
-    return p.group <= 8 ? launch_tile_k<D, STAGES, true>(p, a, segments, st)
-                        : launch_tile_k<D, STAGES, false>(p, a, segments, st);
+    return p.group <= 8 ? launch_bf16<D, true>(p, a, segments, st) : launch_bf16<D, false>(p, a, segments, st);
 }
 
 // ---------------------------------------------------------------------------
-// Any type, block size, head_dim <= 256 and group. A warp takes 32 listed
+// Any type, block size, head_dim <= 256 and group. A warp takes up to 32 listed
 // token slots at a time: each lane finds one slot's address, then the warp
 // goes through them TT tokens per step. Lanes own EPL dimensions of a token's
 // row; the GH x TT partial products of a step are reduced across the lanes so
-// that each lane ends up with one of the scores.
+// that each lane ends up with one of the scores. Where rows are aligned, every
+// lane copies its own dimensions into a ring in shared memory, several steps
+// ahead: no lane reads what another copied, so there is nothing to wait for
+// but a lane's own copies.
 // ---------------------------------------------------------------------------
 
 constexpr int kAnyWarps = 8;
@@ -518,6 +577,27 @@ __device__ __forceinline__ float transpose_sum(float (&v)[NV], uint32_t lane) {
         }
     }
     return v[0];
+}
+
+// x += a * b for N floats, two per instruction, each product and sum rounded
+// as by fmaf.
+template <int N>
+__device__ __forceinline__ void fma_all(float (&x)[N], const float (&a)[N], const float (&b)[N]) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            float2 s = make_float2(x[i], x[i + 1]);
+            const float2 u = make_float2(a[i], a[i + 1]), w = make_float2(b[i], b[i + 1]);
+            asm("fma.rn.f32x2 %0, %1, %2, %0;"
+                : "+l"(reinterpret_cast<unsigned long long&>(s))
+                : "l"(reinterpret_cast<const unsigned long long&>(u)), "l"(reinterpret_cast<const unsigned long long&>(w)));
+            x[i] = s.x;
+            x[i + 1] = s.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = fmaf(a[i], b[i], x[i]);
+    }
 }
 
 // Dimensions a lane owns: EPL in a row where that divides head_dim and the
@@ -556,18 +636,81 @@ __device__ __forceinline__ uint32_t dim_of(uint32_t lane, int i) {
     return VECT ? lane * EPL + i : lane + 32 * i;
 }
 
+// A lane's dimensions of a row, copied by the lane for itself into its own
+// place of a shared-memory row (asynchronously; nobody else reads them).
+template <typename T, int EPL>
+__device__ __forceinline__ void copy_dims(uint32_t place, const T* row, uint32_t D, uint32_t lane) {
+    constexpr int kBytes = EPL * sizeof(T);
+    if (lane * EPL >= D) return;
+    const T* src = row + lane * EPL;
+    if constexpr (kBytes % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place + 512 * i),
+                         "l"(reinterpret_cast<const uint8_t*>(src) + 16 * i)
+                         : "memory");
+    } else if constexpr (kBytes == 8) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(place), "l"(src) : "memory");
+    } else {
+        static_assert(kBytes == 4, "a copy of 4, 8 or 16 bytes");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(place), "l"(src) : "memory");
+    }
+}
+
+// What a lane copied, as floats; zeros where its token is not attended.
+template <typename T, int EPL>
+__device__ __forceinline__ void fetch_dims(float (&x)[EPL], const uint8_t* place, bool live, uint32_t D, uint32_t lane) {
+    constexpr int kBytes = EPL * sizeof(T);
+    if (live && lane * EPL < D) {
+        T raw[EPL];
+        if constexpr (kBytes % 16 == 0) {
+#pragma unroll
+            for (int i = 0; i < kBytes / 16; ++i)
+                reinterpret_cast<uint4*>(raw)[i] = *reinterpret_cast<const uint4*>(place + 512 * i);
+        } else if constexpr (kBytes == 8) {
+            *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(place);
+        } else {
+            *reinterpret_cast<uint32_t*>(raw) = *reinterpret_cast<const uint32_t*>(place);
+        }
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) x[i] = to_float<T>(raw[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) x[i] = 0.f;
+    }
+}
+
+// Steps of TT tokens: a ring of them per warp where rows are copied (VECT).
 template <typename T, int EPL, int GH, bool VECT>
-__global__ void __launch_bounds__(kAnyThreads) decode_selected_any(const SelectedParams p) {
-    constexpr int TT = EPL == 8 || GH == 8 ? 4 : 8;  // tokens per step (their K and V are in registers)
+struct AnyShape {
+    static constexpr int TT = EPL == 8 || GH == 8 ? 4 : 8;
+    static constexpr uint32_t kRow = 32 * EPL * sizeof(T);              // a token's K or V
+    static constexpr uint32_t kStep = TT * 2 * kRow;
+    static constexpr uint32_t kFit = 12 * 1024 / kStep;                 // about 12 KiB of copies in flight per warp
+    static constexpr uint32_t kStages = kFit < 2 ? 2 : kFit > 8 ? 8 : kFit;
+    static constexpr uint32_t kPart = GH * EPL * 32 * sizeof(float);    // a warp's partial output, in the ring's place
+    static constexpr uint32_t kRing = kStages * kStep;
+    static constexpr uint32_t kWarp = VECT && kRing > kPart ? kRing : kPart;
+    static constexpr uint32_t kSmem = kAnyWarps * kWarp;
+};
+
+template <typename T, int EPL, int GH, bool VECT>
+__global__ void __launch_bounds__(kAnyThreads, 2) decode_selected_any(const SelectedParams p) {
+    using S = AnyShape<T, EPL, GH, VECT>;
+    constexpr int TT = S::TT;
     constexpr int NV = GH * TT;
     static_assert(NV <= 32, "a score per lane");
     constexpr int kShift = NV == 32 ? 0 : NV == 16 ? 1 : NV == 8 ? 2 : 3;  // lane >> kShift = tok * GH + head
     constexpr int kHeadBits = GH == 8 ? 3 : GH == 4 ? 2 : GH == 2 ? 1 : 0;
-    __shared__ float part_o[kAnyWarps][GH][EPL * 32];
+    extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float part_m[kAnyWarps][GH], part_l[kAnyWarps][GH];
     __shared__ uint32_t part_seen[kAnyWarps];
     __shared__ float joined_m[GH], joined_l[GH];
     __shared__ uint32_t joined_seen;
+    __shared__ __align__(16) float weights[kAnyWarps][32];
+    auto part_o = [&](uint32_t w, uint32_t g, uint32_t d) -> float* {
+        return reinterpret_cast<float*>(smem + w * S::kWarp) + g * (EPL * 32) + d;
+    };
 
     wait_for_previous_kernel();
     allow_next_kernel();
@@ -626,65 +769,159 @@ __global__ void __launch_bounds__(kAnyThreads) decode_selected_any(const Selecte
     };
     uint64_t s0 = static_cast<uint64_t>(rank * kAnyWarps + warp) * p.round;
     const T* next = row_of(s0 + lane);
-    for (; s0 < slots; s0 += stride) {
-        const T* mine = next;
-        next = row_of(s0 + stride + lane);
-        const uint32_t valid = __ballot_sync(0xffffffffu, mine != nullptr);
-        seen += __popc(valid);
-        for (uint32_t t0 = 0; t0 < p.round; t0 += TT) {
-            if (((valid >> t0) & ((1ull << TT) - 1)) == 0) continue;
-            float k[TT][EPL], v[TT][EPL];
+
+    // One step: token t of it is attended where bit t of `valid` is set;
+    // fetch(x, t, v) gives this lane's dimensions of its K (v = 0) or V.
+    auto step = [&](uint32_t valid, auto fetch) {
+        float s[NV];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                const T* at = reinterpret_cast<const T*>(
-                    __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), t0 + t));
-                if (at != nullptr) {
-                    load_dims<T, EPL, VECT>(k[t], at, p.D, lane);
-                    load_dims<T, EPL, VECT>(v[t], at + p.T * row, p.D, lane);
-                } else {
+        for (int t = 0; t < TT; ++t) {
+            float k[EPL];
+            fetch(k, t, 0);
 #pragma unroll
-                    for (int i = 0; i < EPL; ++i) k[t][i] = v[t][i] = 0.f;
+            for (int g = 0; g < GH; ++g) {
+                // two sums (of even and odd dimensions) where there are two
+                constexpr int N = EPL % 2 == 0 ? 2 : 1;
+                float x[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) x[i] = q[g][i] * k[i];
+#pragma unroll
+                for (int i = N; i < EPL; i += N) {
+                    float a[N], b[N];
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        a[j] = q[g][i + j];
+                        b[j] = k[i + j];
+                    }
+                    fma_all<N>(x, a, b);
                 }
+                s[t * GH + g] = N == 2 ? x[0] + x[N - 1] : x[0];
             }
-            float s[NV];
+        }
+        float x = transpose_sum<NV>(s, lane);
+        const uint32_t tok = lane >> (kShift + kHeadBits);
+        if (!((valid >> tok) & 1u)) x = -INFINITY;
+        float top = x;
 #pragma unroll
-            for (int t = 0; t < TT; ++t)
+        for (int off = 1 << (kShift + kHeadBits); off < 32; off <<= 1)
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float m_new = fmaxf(m, top);
+        const float m_ref = m_new == -INFINITY ? 0.f : m_new;  // nothing above -inf yet: weights are 0, not NaN
+        const float e = exp2f(x - m_ref);
+        const float corr = exp2f(m - m_ref);
+        l = l * corr + e;
+        if (__any_sync(0xffffffffu, m_new > m)) {
 #pragma unroll
-                for (int g = 0; g < GH; ++g) {
-                    float x = 0.f;
+            for (int g = 0; g < GH; ++g) {
+                const float c = __shfl_sync(0xffffffffu, corr, g << kShift);
 #pragma unroll
-                    for (int i = 0; i < EPL; ++i) x += q[g][i] * k[t][i];
-                    s[t * GH + g] = x;
-                }
-            float x = transpose_sum<NV>(s, lane);
-            const uint32_t tok = lane >> (kShift + kHeadBits);
-            if (!((valid >> (t0 + tok)) & 1u)) x = -INFINITY;
-            float top = x;
-#pragma unroll
-            for (int off = 1 << (kShift + kHeadBits); off < 32; off <<= 1)
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            const float m_new = fmaxf(m, top);
-            const float m_ref = m_new == -INFINITY ? 0.f : m_new;  // nothing above -inf yet: weights are 0, not NaN
-            const float e = exp2f(x - m_ref);
-            const float corr = exp2f(m - m_ref);
-            l = l * corr + e;
-            if (__any_sync(0xffffffffu, m_new > m)) {
-#pragma unroll
-                for (int g = 0; g < GH; ++g) {
-                    const float c = __shfl_sync(0xffffffffu, corr, g << kShift);
-#pragma unroll
-                    for (int i = 0; i < EPL; ++i) o[g][i] *= c;
-                }
+                for (int i = 0; i < EPL; ++i) o[g][i] *= c;
             }
-            m = m_new;
+        }
+        m = m_new;
+        // every lane needs every weight: through shared memory
+        __syncwarp();  // the weights of the step before have been read
+        if ((lane & ((1u << kShift) - 1)) == 0) weights[warp][lane >> kShift] = e;
+        __syncwarp();
 #pragma unroll
-            for (int t = 0; t < TT; ++t)
+        for (int t = 0; t < TT; ++t) {
+            float v[EPL];
+            __align__(16) float w[GH];
+            fetch(v, t, 1);
+            if constexpr (GH % 4 == 0) {
 #pragma unroll
-                for (int g = 0; g < GH; ++g) {
-                    const float w = __shfl_sync(0xffffffffu, e, (t * GH + g) << kShift);
+                for (int g = 0; g < GH; g += 4)
+                    *reinterpret_cast<float4*>(&w[g]) = *reinterpret_cast<const float4*>(&weights[warp][t * GH + g]);
+            } else {
 #pragma unroll
-                    for (int i = 0; i < EPL; ++i) o[g][i] += w * v[t][i];
+                for (int g = 0; g < GH; ++g) w[g] = weights[warp][t * GH + g];
+            }
+#pragma unroll
+            for (int g = 0; g < GH; ++g) {
+                float ws[EPL];
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) ws[i] = w[g];
+                fma_all<EPL>(o[g], ws, v);
+            }
+        }
+    };
+    constexpr uint32_t kStepBits = (1u << TT) - 1u;
+    if constexpr (VECT) {
+        // the round that is being copied: this lane's row, the steps left of it
+        const T* mine = nullptr;
+        uint32_t valid = 0, t0 = 0;
+        uint64_t valid_of = 0;                      // of each slot of the ring, 8 bits each
+        uint32_t issued = 0, used = 0;
+        const uint8_t* ring = smem + warp * S::kWarp + lane * (S::kRow / 32 < 16 ? S::kRow / 32 : 16);
+        const uint32_t ring_at = smem_u32(ring);
+        bool more = true;
+        // Copies the next step with a token to attend; a group of copies per
+        // call, empty past the last, so that the waits count.
+        auto issue = [&]() {
+            while (more && ((valid >> t0) & kStepBits) == 0) {
+                t0 += TT;
+                if (t0 < p.round && valid >> t0 != 0) continue;
+                more = s0 < slots;
+                if (!more) break;
+                mine = next;
+                valid = __ballot_sync(0xffffffffu, mine != nullptr);
+                seen += __popc(valid);
+                t0 = 0;
+                s0 += stride;
+                next = row_of(s0 + lane);
+            }
+            if (more) {
+                const uint32_t slot = issued % S::kStages, bits = (valid >> t0) & kStepBits;
+                const uint32_t to = ring_at + slot * S::kStep;
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    const T* at = reinterpret_cast<const T*>(
+                        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), t0 + t));
+                    if (at != nullptr) {
+                        copy_dims<T, EPL>(to + (2 * t) * S::kRow, at, p.D, lane);
+                        copy_dims<T, EPL>(to + (2 * t + 1) * S::kRow, at + p.T * row, p.D, lane);
+                    }
                 }
+                valid_of = (valid_of & ~(0xffull << (8 * slot))) | (static_cast<uint64_t>(bits) << (8 * slot));
+                valid &= ~(kStepBits << t0);
+                ++issued;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        for (uint32_t i = 0; i + 1 < S::kStages; ++i) issue();
+        for (;;) {
+            issue();
+            if (used == issued) break;
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+            const uint32_t slot = used % S::kStages;
+            const uint32_t bits = static_cast<uint32_t>(valid_of >> (8 * slot)) & kStepBits;
+            step(bits, [&](float (&x)[EPL], int t, int v) {
+                fetch_dims<T, EPL>(x, ring + slot * S::kStep + (2 * t + v) * S::kRow, (bits >> t) & 1u, p.D, lane);
+            });
+            ++used;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();  // the ring becomes this warp's partial output
+    } else {
+        for (; s0 < slots; s0 += stride) {
+            const T* mine = next;
+            next = row_of(s0 + stride + lane);
+            const uint32_t valid = __ballot_sync(0xffffffffu, mine != nullptr);
+            seen += __popc(valid);
+            for (uint32_t t0 = 0; t0 < p.round; t0 += TT) {
+                const uint32_t bits = (valid >> t0) & kStepBits;
+                if (bits == 0) continue;
+                step(bits, [&](float (&x)[EPL], int t, int v) {
+                    const T* at = reinterpret_cast<const T*>(
+                        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), t0 + t));
+                    if (at != nullptr) {
+                        load_dims<T, EPL, false>(x, at + v * p.T * row, p.D, lane);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < EPL; ++i) x[i] = 0.f;
+                    }
+                });
+            }
         }
     }
 #pragma unroll
@@ -694,7 +931,7 @@ __global__ void __launch_bounds__(kAnyThreads) decode_selected_any(const Selecte
 #pragma unroll
     for (int g = 0; g < GH; ++g)
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) part_o[warp][g][dim_of<EPL, VECT>(lane, i)] = o[g][i];
+        for (int i = 0; i < EPL; ++i) *part_o(warp, g, dim_of<EPL, VECT>(lane, i)) = o[g][i];
     if (lane < (GH << kShift) && (lane & ((1u << kShift) - 1)) == 0) {
         part_m[warp][lane >> kShift] = m;
         part_l[warp][lane >> kShift] = l;
@@ -720,12 +957,12 @@ __global__ void __launch_bounds__(kAnyThreads) decode_selected_any(const Selecte
         for (int w = 0; w < kAnyWarps; ++w) {
             const float c = partial_weight(part_m[w][g], M);
             sum += c * part_l[w][g];
-            acc += c * part_o[w][g][d];
+            acc += c * *part_o(w, g, d);
         }
         if (cluster == 1) {
             write_out(g, d, acc, sum);
         } else {
-            part_o[0][g][d] = acc;
+            *part_o(0, g, d) = acc;
             if (d == 0) {
                 joined_m[g] = M;
                 joined_l[g] = sum;
@@ -746,7 +983,7 @@ __global__ void __launch_bounds__(kAnyThreads) decode_selected_any(const Selecte
             if (r < cluster) {
                 m[r] = *cl.map_shared_rank(&joined_m[g], r);
                 l[r] = *cl.map_shared_rank(&joined_l[g], r);
-                o[r] = *cl.map_shared_rank(&part_o[0][g][d], r);
+                o[r] = *cl.map_shared_rank(part_o(0, g, d), r);
                 any |= *cl.map_shared_rank(&joined_seen, r);
             }
             M = fmaxf(M, m[r]);
@@ -764,14 +1001,24 @@ __global__ void __launch_bounds__(kAnyThreads) decode_selected_any(const Selecte
     cl.sync();
 }
 
+template <typename T, int EPL, int GH, bool VECT>
+int launch_any_v(const SelectedParams& p, uint32_t segments, cudaStream_t st) {
+    using S = AnyShape<T, EPL, GH, VECT>;
+    static std::atomic<std::uint64_t> attr_done{0};
+    auto kern = decode_selected_any<T, EPL, GH, VECT>;
+    const int rc = set_smem_limit_once(attr_done, reinterpret_cast<const void*>(kern), S::kSmem,
+                                       "cudaFuncSetAttribute(decode_selected)");
+    if (rc != QVP_OK) return rc;
+    const dim3 grid(segments * p.cluster, ceil_div(p.group, GH));
+    return launch_dependent("launch decode_selected", kern, grid, kAnyThreads, S::kSmem, p.cluster, st, p);
+}
+
 template <typename T, int EPL, int GH>
 int launch_any_t(const SelectedParams& p, bool vect, uint32_t segments, cudaStream_t st) {
-    const dim3 grid(segments * p.cluster, ceil_div(p.group, GH));
-    if (vect)
-        return launch_dependent("launch decode_selected", decode_selected_any<T, EPL, GH, true>, grid, kAnyThreads, 0,
-                                p.cluster, st, p);
-    return launch_dependent("launch decode_selected", decode_selected_any<T, EPL, GH, false>, grid, kAnyThreads, 0,
-                            p.cluster, st, p);
+    if constexpr (EPL * sizeof(T) >= 4) {  // the smallest asynchronous copy
+        if (vect) return launch_any_v<T, EPL, GH, true>(p, segments, st);
+    }
+    return launch_any_v<T, EPL, GH, false>(p, segments, st);
 }
 
 template <typename T, int EPL>
@@ -856,20 +1103,20 @@ extern "C" int qvp_decode_selected(const qvp_decode_selected_args* args, qvp_str
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const uint64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
     const bool tile = a.dtype == QVP_DTYPE_BF16 && (p.D == 64 || p.D == 96 || p.D == 128) &&
-                      (p.T % 16 == 0 || p.T == 8) &&
-                      a.block_stride == qvp_block_bytes(&sh) && aligned_to(a.pool, 16) && aligned_to(a.query, 4) &&
-                      q_pitch % 2 == 0 && aligned_to(a.out, 4) &&
+                      (p.T % 16 == 0 || p.T == 8) && a.block_stride == qvp_block_bytes(&sh) && aligned_to(a.pool, 16) &&
+                      aligned_to(a.query, 4) && q_pitch % 2 == 0 && aligned_to(a.out, 4) &&
                       static_cast<uint64_t>(a.num_blocks) * sh.num_layers * 2 * p.T < (1ull << 31);
     if (tile) {
         const uint64_t pieces = (static_cast<uint64_t>(p.keep) * p.T + 15) / 16;
         p.cluster = 1;
-        // two CTAs are resident per SM: split a list while the whole grid still is
+        // Two CTAs are resident per SM: split a list while the whole grid still
+        // is (256 lists of 128 blocks: 47 us whole, 52 us in two; 8 lists of
+        // 128 blocks: 25 us whole, 8.4 us in eight).
         while (p.cluster < kMaxCluster && segments * p.cluster * 2 <= 2 * sms && pieces > kTileWarps * p.cluster)
             p.cluster *= 2;
-        // 24 KiB of copies in flight per warp
-        return p.D == 128  ? launch_tile<128, 3>(p, a, static_cast<uint32_t>(segments), st)
-               : p.D == 96 ? launch_tile<96, 4>(p, a, static_cast<uint32_t>(segments), st)
-                           : launch_tile<64, 6>(p, a, static_cast<uint32_t>(segments), st);
+        return p.D == 128  ? launch_tile<128>(p, a, static_cast<uint32_t>(segments), st)
+               : p.D == 96 ? launch_tile<96>(p, a, static_cast<uint32_t>(segments), st)
+                           : launch_tile<64>(p, a, static_cast<uint32_t>(segments), st);
     }
     const uint64_t slots = static_cast<uint64_t>(p.keep) * p.T;
     p.cluster = 1;

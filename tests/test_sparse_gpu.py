@@ -616,6 +616,32 @@ def test_attend_scores_of_minus_infinity(dtype, D):
     near_attention(c, out[:1], q[:1], lists[:1], ctx=c.ctx[:1])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("D,hq", [(64, 4), (96, 4), (128, 8), (128, 16), (80, 4), (33, 2)])
+def test_attend_infinities_and_nan_stay_where_they_are(dtype, D, hq):
+    """An infinity or NaN of V reaches its dimension of the heads that attend it, and no other."""
+    torch = _torch()
+    c = Cache(36, [160, 320, 160], dtype=dtype, hkv=1, D=D)
+    q = c.make((3, hq, D))
+    clean = np.broadcast_to(np.arange(10, dtype=np.int32), (3, 1, 10)).copy()
+    args, out = c.attend_args(q, torch.from_numpy(clean).cuda())
+    assert qvp.decode_selected(args, _stream()) == qvp.OK
+    want = out.double().cpu().numpy()
+    v = c.pool[:, :c.n].unflatten(1, (2, 16, 1, D))[:, 1]
+    for block, slot, dim, x in ((0, 3, 1, math.inf), (4, 15, 5, -math.inf), (7, 0, D - 1, math.nan)):
+        v[int(c.tables[0, block]), slot, 0, dim] = x
+        want[0, :, dim] = x
+    v[int(c.tables[1, 15]), :, 0, 2] = math.inf  # not listed
+    assert qvp.decode_selected(args, _stream()) == qvp.OK and c.errors() == 0
+    got = out.double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), np.isinf(want))
+    fine = np.isfinite(want)
+    assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    # both results of a finite element are within the bound of the same exact value: weights of one bf16 term,
+    # values below 6, and the rounding of each result
+    assert np.abs(got[fine] - want[fine]).max() < (2 * (2.0**-8 + 2.0**-9) * 6 if dtype == "bf16" else 1e-4)
+
+
 @pytest.mark.parametrize("what,bit", [("past", 1), ("id", 1), ("long", 4), ("negative", 4)])
 @pytest.mark.parametrize("D", [128, 96])
 def test_attend_flags_bad_entries_and_serves_the_rest(what, bit, D):
