@@ -109,8 +109,12 @@ struct TileShape {
     static constexpr uint32_t kRing = kStages * kPiece;              // one warp's
     static constexpr uint32_t kBars = kTileWarps * kRing;            // offset of the barriers
     static constexpr uint32_t kStats = kBars + kTileWarps * kStages * 8;  // m, l of 16 rows per warp, tokens seen
-    static constexpr uint32_t kJoined = kStats + kTileWarps * (32 * 4 + 16);  // the same of the whole CTA
-    static constexpr uint32_t kSmem = kJoined + 32 * 4 + 16 + 1024;
+    // of every CTA of a cluster: m and l of its rows, and its sums of the
+    // columns that this CTA writes out
+    static constexpr uint32_t kRanks = kStats + kTileWarps * (32 * 4 + 16);
+    static constexpr uint32_t kShare = kRanks + kMaxCluster * Tile::kHeads * 8;
+    static constexpr uint32_t kPairs = Tile::kHeads * Tile::kDim / 2;
+    static constexpr uint32_t kSmem = kShare + (kPairs + kMaxCluster * kMaxCluster) * 8 + 1024;
     static_assert(kRing >= Tile::kHeads * Tile::kDim * 4, "a warp's partial output takes the place of its ring");
     static_assert(kPiece % 1024 == 0 && kStages <= 8, "pieces start on swizzle boundaries, their counts fit 64 bits");
 };
@@ -126,18 +130,19 @@ __device__ __forceinline__ void attend_piece(WarpState<D>& st, const uint32_t (&
     const int c = lane & 3;
     const int mi = lane >> 3;
     const int li = lane & 7;
-    float s[2][4];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) s[a][0] = s[a][1] = s[a][2] = s[a][3] = 0.f;
-    // the lane's row and swizzle are the same in every step: at(chunk) differs
-    // by a constant and the chunk's bits
+    // even and odd steps apart, for shorter chains of dependent products
+    float s[2][4] = {}, odd[2][4] = {};
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
         uint32_t r0, r1, r2, r3;
         ldmatrix_x4(L::at(piece, 2 * ks + (mi & 1), mi >> 1, li), r0, r1, r2, r3);
-        mma_bf16_16816(s[0], qa[ks], r0, r1);
-        mma_bf16_16816(s[1], qa[ks], r2, r3);
+        mma_bf16_16816(ks % 2 == 0 ? s[0] : odd[0], qa[ks], r0, r1);
+        mma_bf16_16816(ks % 2 == 0 ? s[1] : odd[1], qa[ks], r2, r3);
     }
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[a][e] += odd[a][e];
     constexpr int kRows = PAIR ? 1 : 2;
     uint32_t pa[4];
     float corr[2] = {1.f, 1.f};
@@ -211,6 +216,7 @@ struct Bf16Tile {
     static constexpr int kHalf = PieceLayout<D, KIND>::kHalf;
 
     static constexpr bool kSplits = PAIR;
+    static constexpr bool kParts = KIND == kPart;                     // a block may have several pieces
 
     uint32_t qa[D / 16][4];
     WarpState<D> st;
@@ -306,26 +312,27 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         mbar_fence_init();
     }
     __syncwarp();
+    const uint32_t cluster = p.cluster;
+    if (cluster > 1) cg::this_cluster().barrier_arrive();
     wait_for_previous_kernel();
     allow_next_kernel();
 
-    const uint32_t cluster = p.cluster;
     const uint32_t rank = blockIdx.x % cluster, seg = blockIdx.x / cluster;
     const uint32_t b = seg / p.hkv, head = seg % p.hkv;
     const int G = static_cast<int>(min(p.group - blockIdx.y * Tile::kHeads, static_cast<uint32_t>(Tile::kHeads)));
     const size_t h0 = static_cast<size_t>(head) * p.group + blockIdx.y * Tile::kHeads;
     const int32_t* list = p.selected + static_cast<size_t>(seg) * p.keep;
     const int32_t* table = p.tables + static_cast<size_t>(b) * p.pitch;
-    const uint32_t per_block = kBlocks == 1 ? p.T / 16 : 1;  // pieces of a block
-    const uint64_t pieces = (static_cast<uint64_t>(p.keep) * per_block + kBlocks - 1) / kBlocks;
+    const uint32_t per_block = Tile::kParts ? p.T / 16 : 1;        // pieces of a block
+    const uint32_t pieces = (p.keep * per_block + kBlocks - 1) / kBlocks;
     const uint32_t workers = cluster * kTileWarps, worker = rank * kTileWarps + warp;
     // The lane's piece of a window of 32 per warp: its listed blocks (-1:
     // none) and their frames. Neither load waits for the context length.
     int32_t blk[kBlocks], frame[kBlocks];
-    auto load_blocks = [&](uint64_t i) {
+    auto load_blocks = [&](uint32_t i) {
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) {
-            const uint64_t e = kBlocks * (i / per_block) + k;
+            const uint32_t e = kBlocks * (Tile::kParts ? i / per_block : i) + k;
             blk[k] = e < p.keep ? list[e] : -1;
         }
     };
@@ -333,7 +340,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) frame[k] = static_cast<uint32_t>(blk[k]) < p.pitch ? table[blk[k]] : -1;
     };
-    uint64_t mine = worker + static_cast<uint64_t>(workers) * lane;
+    uint32_t mine = worker + workers * lane;
     load_blocks(mine);
     const int ctx = p.ctx[b];
 
@@ -342,6 +349,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     load_frames();
     if (ctx < 0 || static_cast<uint32_t>(ctx) > p.capacity) {  // the whole cluster
         if (threadIdx.x == 0) record_error(p.err, kErrBadContext);
+        if (cluster > 1) cg::this_cluster().barrier_wait();
         return;
     }
     const uint32_t nblk = (static_cast<uint32_t>(ctx) + p.T - 1) / p.T;
@@ -354,9 +362,9 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     // of its halves, and the lanes whose pieces are still to be copied
     int krow[kBlocks], va = 0, vb = 0;
     uint32_t to_issue = 0;
-    uint64_t base = worker;                 // the next window's first piece
+    uint32_t base = worker;                 // the next window's first piece
     auto next_window = [&]() {
-        const uint32_t first = static_cast<uint32_t>(mine % per_block) * 16;
+        const uint32_t first = Tile::kParts ? mine % per_block * 16 : 0;
         int left[kBlocks];                  // tokens from the piece's first to the context's end
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) {
@@ -375,8 +383,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         va = max(0, min(8, left[0]));
         vb = max(0, min(8, kBlocks == 2 ? left[kBlocks - 1] : left[0] - 8));
         to_issue = __ballot_sync(0xffffffffu, va + vb > 0);
-        base += static_cast<uint64_t>(workers) * 32;
-        mine += static_cast<uint64_t>(workers) * 32;
+        base += workers * 32;
+        mine += workers * 32;
         load_blocks(mine);                  // of the window after it
         load_frames();
     };
@@ -424,7 +432,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         tile.restart();
         seen = 0;
         base = worker;
-        mine = worker + static_cast<uint64_t>(workers) * lane;
+        mine = worker + workers * lane;
         load_blocks(mine);
         load_frames();
     }
@@ -441,7 +449,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     }
     __syncthreads();
     // Join the warps, two elements a thread: straight to the output, or to the
-    // first warp's place for the cluster.
+    // CTA of the cluster that writes them out. A CTA that attended no token
+    // says so by a negative sum.
     const float* stats = reinterpret_cast<const float*>(smem + S::kStats);
     T* out = static_cast<T*>(p.out) + (static_cast<size_t>(b) * p.hq + h0) * D;
     uint32_t any = 0;
@@ -449,9 +458,12 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     for (int w = 0; w < kTileWarps; ++w) any |= reinterpret_cast<const uint32_t*>(stats)[w * 36 + 32];
     auto write_out = [&](uint32_t g, uint32_t d, float x, float y, float sum) {
         const float inv = 1.f / sum;
-        *reinterpret_cast<uint32_t*>(out + g * D + d) = any != 0 ? pack_bf16x2(x * inv, y * inv) : 0u;
+        *reinterpret_cast<uint32_t*>(out + g * D + d) = sum < 0.f ? 0u : pack_bf16x2(x * inv, y * inv);
     };
-    for (uint32_t i = threadIdx.x; i < static_cast<uint32_t>(G) * (D / 2); i += kTileThreads) {
+    const uint32_t pairs = static_cast<uint32_t>(G) * (D / 2);
+    const uint32_t share = (pairs + cluster - 1) / cluster;  // pairs that a CTA writes out
+    if (cluster > 1) cg::this_cluster().barrier_wait();      // every CTA has started: its memory can be written
+    for (uint32_t i = threadIdx.x; i < pairs; i += kTileThreads) {
         const uint32_t g = i / (D / 2), d = i % (D / 2) * 2;
         float M = -INFINITY;
 #pragma unroll
@@ -465,54 +477,41 @@ __global__ void __launch_bounds__(kTileThreads, 2)
             x += weight * o.x;
             y += weight * o.y;
         }
+        if (any == 0) sum = -1.f;
         if (cluster == 1) {
             write_out(g, d, x, y, sum);
         } else {
-            *reinterpret_cast<float2*>(smem + (g * D + d) * 4) = make_float2(x, y);
-            if (d == 0) {
-                float* joined = reinterpret_cast<float*>(smem + S::kJoined);
-                joined[g] = M;
-                joined[16 + g] = sum;
-                if (g == 0) reinterpret_cast<uint32_t*>(joined)[32] = any;
-            }
+            uint8_t* to = cg::this_cluster().map_shared_rank(smem, i / share);
+            reinterpret_cast<float2*>(to + S::kShare)[rank * share + i % share] = make_float2(x, y);
+            if (d == 0)
+                for (uint32_t r = 0; r < cluster; ++r)
+                    reinterpret_cast<float2*>(cg::this_cluster().map_shared_rank(smem, r) +
+                                              S::kRanks)[rank * Tile::kHeads + g] = make_float2(M, sum);
         }
     }
     if (cluster == 1) return;
-    cg::cluster_group cl = cg::this_cluster();
-    cl.sync();
-    for (uint32_t i = rank * kTileThreads + threadIdx.x; i < static_cast<uint32_t>(G) * (D / 2);
-         i += cluster * kTileThreads) {
+    cg::this_cluster().sync();
+    for (uint32_t k = threadIdx.x; k < share; k += kTileThreads) {
+        const uint32_t i = rank * share + k;
+        if (i >= pairs) break;
         const uint32_t g = i / (D / 2), d = i % (D / 2) * 2;
-        float m[kMaxCluster], l[kMaxCluster];
-        float2 o[kMaxCluster];
+        const float2* rows = reinterpret_cast<const float2*>(smem + S::kRanks);
+        const float2* sums = reinterpret_cast<const float2*>(smem + S::kShare);
         float M = -INFINITY;
-#pragma unroll
-        for (uint32_t r = 0; r < kMaxCluster; ++r) {
-            m[r] = -INFINITY;
-            l[r] = 0.f;
-            o[r] = make_float2(0.f, 0.f);
-            if (r < cluster) {
-                const uint8_t* at = cl.map_shared_rank(smem, r);
-                const float* joined = reinterpret_cast<const float*>(at + S::kJoined);
-                m[r] = joined[g];
-                l[r] = joined[16 + g];
-                any |= reinterpret_cast<const uint32_t*>(joined)[32];
-                o[r] = *reinterpret_cast<const float2*>(at + (g * D + d) * 4);
-            }
-            M = fmaxf(M, m[r]);
-        }
+        for (uint32_t r = 0; r < cluster; ++r) M = fmaxf(M, rows[r * Tile::kHeads + g].x);
         float sum = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-        for (uint32_t r = 0; r < kMaxCluster; ++r) {
-            const float weight = partial_weight(m[r], M);
-            sum += weight * l[r];
-            x += weight * o[r].x;
-            y += weight * o[r].y;
+        bool none = true;
+        for (uint32_t r = 0; r < cluster; ++r) {
+            const float2 row = rows[r * Tile::kHeads + g], o = sums[r * share + k];
+            if (row.y < 0.f) continue;
+            const float weight = partial_weight(row.x, M);
+            none = false;
+            sum += weight * row.y;
+            x += weight * o.x;
+            y += weight * o.y;
         }
-        write_out(g, d, x, y, sum);
+        write_out(g, d, x, y, none ? -1.f : sum);
     }
-    // no CTA leaves while another may read its shared memory
-    cl.sync();
 }
 
 template <typename Tile>
@@ -1076,7 +1075,10 @@ extern "C" int qvp_decode_selected(const qvp_decode_selected_args* args, qvp_str
     const size_t q_pitch = a.query_pitch != 0 ? a.query_pitch : q_row;
     if (q_pitch < q_row) return fail(QVP_ERR_INVALID, "query pitch below a token's row");
     const uint64_t segments = static_cast<uint64_t>(a.batch) * sh.num_kv_heads;
-    if (segments > 0x7fffffffu) return fail(QVP_ERR_UNSUPPORTED, "more than 2^31 sequences and heads");
+    if (segments > 0x7fffffffu / kMaxCluster)
+        return fail(QVP_ERR_UNSUPPORTED, "more than 2^28 sequences and heads");
+    if (static_cast<uint64_t>(a.max_selected) * sh.tokens_per_block > 0x7fffffffu)
+        return fail(QVP_ERR_UNSUPPORTED, "lists of more than 2^31 tokens");
 
     SelectedParams p;
     p.pool = static_cast<const uint8_t*>(a.pool);
