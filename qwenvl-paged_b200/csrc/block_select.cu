@@ -514,23 +514,39 @@ __device__ uint32_t take_best(const SelectParams& p, const SelectPart& part, uin
     return at;
 }
 
-// Sums over the query heads of the group: [down D | up D].
+// Sums over the query heads of the group: [down D | up D]. A thread's first
+// kAhead heads of its first dimension are loaded by `load`, so that other loads
+// can be issued before `store` needs them.
 template <typename T>
-__device__ __forceinline__ void make_weights(const SelectParams& p, uint32_t b, uint32_t head, double* weight) {
-    for (uint32_t d = threadIdx.x; d < p.D; d += kSelThreads) {
-        const T* q = static_cast<const T*>(p.q) + b * p.q_pitch + static_cast<size_t>(head) * p.group * p.D + d;
-        double up = 0.0, down = 0.0;
-#pragma unroll 8
-        for (uint32_t g = 0; g < p.group; ++g) {
-            const double x = static_cast<double>(to_float<T>(q[static_cast<size_t>(g) * p.D]));
-            // a NaN goes to both sums
-            if (!(x < 0.0)) up += x;
-            if (!(x > 0.0)) down += x;
-        }
-        weight[d] = down;
-        weight[p.D + d] = up;
+struct Weights {
+    static constexpr uint32_t kAhead = 8;
+    const T* q;
+    T first[kAhead];
+
+    __device__ __forceinline__ void load(const SelectParams& p, uint32_t b, uint32_t head) {
+        q = static_cast<const T*>(p.q) + b * p.q_pitch + static_cast<size_t>(head) * p.group * p.D;
+#pragma unroll
+        for (uint32_t g = 0; g < kAhead; ++g)
+            if (threadIdx.x < p.D && g < p.group) first[g] = q[g * p.D + threadIdx.x];
     }
-}
+    __device__ __forceinline__ void store(const SelectParams& p, double* weight) const {
+        for (uint32_t d = threadIdx.x; d < p.D; d += kSelThreads) {
+            double up = 0.0, down = 0.0;
+            auto add = [&](T value) {
+                const double x = static_cast<double>(to_float<T>(value));
+                // a NaN goes to both sums
+                if (!(x < 0.0)) up += x;
+                if (!(x > 0.0)) down += x;
+            };
+#pragma unroll
+            for (uint32_t g = 0; g < kAhead; ++g)
+                if (g < p.group) add(first[g]);
+            for (uint32_t g = kAhead; g < p.group; ++g) add(q[static_cast<size_t>(g) * p.D + d]);
+            weight[d] = down;
+            weight[p.D + d] = up;
+        }
+    }
+};
 
 // The weights as three bf16 terms each, what the terms before leave of a
 // weight, rounded, and the size of the first: [4][PITCH].
@@ -691,18 +707,16 @@ __device__ __forceinline__ double score_tiles(const SelectParams& p, const Selec
         id0 = id_of(base + row);
         id1 = id_of(base + row + 8);
     }
-    make_weights<T>(p, b, part.head, weight);
-    __syncthreads();
-    split_weights<kPitch>(p, weight, terms);
-    __syncthreads();
-    const T* columns = terms + row * kPitch + col * 8;
-#pragma unroll 1
-    for (; base < n; base += kStride) {
-        const bool bad0 = static_cast<uint32_t>(id0) >= p.num_blocks, bad1 = static_cast<uint32_t>(id1) >= p.num_blocks;
+    Weights<T> weights;
+    weights.load(p, b, part.head);
+    uint4 x[LOADS], y[LOADS];
+    bool bad0 = false, bad1 = false;
+    auto load = [&]() {
+        bad0 = static_cast<uint32_t>(id0) >= p.num_blocks;
+        bad1 = static_cast<uint32_t>(id1) >= p.num_blocks;
         if (bad0 || bad1) record_error(p.err, kErrBadBlockId);
         const T* at0 = rows + static_cast<size_t>(bad0 ? 0 : id0) * stride;
         const T* at1 = rows + static_cast<size_t>(bad1 ? 0 : id1) * stride;
-        uint4 x[LOADS], y[LOADS];
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
             x[j] = *reinterpret_cast<const uint4*>(at0 + j * 32);
@@ -710,6 +724,17 @@ __device__ __forceinline__ double score_tiles(const SelectParams& p, const Selec
         }
         id0 = id_of(base + kStride + row);
         id1 = id_of(base + kStride + row + 8);
+    };
+    if (base < n) load();
+    // the first rows are on their way
+    weights.store(p, weight);
+    __syncthreads();
+    split_weights<kPitch>(p, weight, terms);
+    __syncthreads();
+    const T* columns = terms + row * kPitch + col * 8;
+#pragma unroll 1
+    for (bool first = true; base < n; base += kStride, first = false) {
+        if (!first) load();
         float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
         float size_even[4] = {0.f, 0.f, 0.f, 0.f}, size_odd[4] = {0.f, 0.f, 0.f, 0.f};
         constexpr uint32_t kSize = 0x7fff7fffu;
@@ -757,7 +782,9 @@ struct ByTile {};
 template <typename T>
 __device__ __forceinline__ double score_part(ByElement, const SelectParams& p, const SelectPart& part, uint32_t b,
                                              double* weight, float& lo, float& hi, float&) {
-    make_weights<T>(p, b, part.head, weight);
+    Weights<T> weights;
+    weights.load(p, b, part.head);
+    weights.store(p, weight);
     __syncthreads();
     score_each<T>(p, part, lo, hi);
     return 0.0;
@@ -765,7 +792,9 @@ __device__ __forceinline__ double score_part(ByElement, const SelectParams& p, c
 template <typename T, int LANES, int VECS>
 __device__ __forceinline__ double score_part(ByVector<LANES, VECS>, const SelectParams& p, const SelectPart& part,
                                              uint32_t b, double* weight, float& lo, float& hi, float&) {
-    make_weights<T>(p, b, part.head, weight);
+    Weights<T> weights;
+    weights.load(p, b, part.head);
+    weights.store(p, weight);
     __syncthreads();
     score_vectors<T, LANES, VECS>(p, part, lo, hi);
     return 0.0;
