@@ -124,6 +124,9 @@ inline int check_shape(const qvp_block_shape& sh, int32_t dtype, uint32_t layer)
     // table capacities are compared as 32-bit token counts on the device
     if (sh.tokens_per_block > 65536u || sh.num_kv_heads > 65535u)
         return fail(QVP_ERR_UNSUPPORTED, "blocks of more than 65536 tokens or 65535 heads");
+    // elements within a block's K are counted in 32 bits
+    if (static_cast<uint64_t>(sh.tokens_per_block) * sh.num_kv_heads * sh.head_dim > 0x7fffffffu)
+        return fail(QVP_ERR_UNSUPPORTED, "blocks of more than 2^31 - 1 elements of K in a layer");
     return QVP_OK;
 }
 

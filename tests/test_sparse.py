@@ -123,6 +123,18 @@ def test_what_the_kernels_do_not_cover_is_refused(call):
     assert call(batch=0) == qvp.OK  # nothing to do: no launch
 
 
+@pytest.mark.parametrize("call,pool", [(_append, True), (_summarize, True), (_select, False), (_attend, True)])
+def test_blocks_past_32_bits_of_elements_are_refused(call, pool):
+    huge = qvp.make_shape(65536, 1, 512, 128, 2)
+    where = dict(block_stride=qvp.block_stride(huge)) if pool else {}
+    if call is not _attend:
+        where["summary_stride"] = qvp.block_stride(qvp.summary_shape(huge))
+    if call is not _summarize:
+        where["num_query_heads"] = 512
+    assert call(shape=huge, layer=0, **where) == qvp.ERR_UNSUPPORTED
+    assert "elements" in qvp.last_error()
+
+
 def test_select_refuses_contexts_that_do_not_fit_a_cluster():
     blocks = 8 * 20480 + 2
     assert _select(max_blocks_per_seq=blocks + 1, max_context_len=(blocks + 1) * 16) == qvp.ERR_UNSUPPORTED
