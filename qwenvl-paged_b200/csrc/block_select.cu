@@ -913,6 +913,7 @@ extern "C" int qvp_select_blocks(const qvp_select_args* args, qvp_stream_t strea
     if (a.max_selected == 0) return fail(QVP_ERR_INVALID, "max_selected is zero");
     if (static_cast<uint64_t>(a.sink_blocks) + a.recent_blocks > a.max_selected)
         return fail(QVP_ERR_INVALID, "sink_blocks and recent_blocks exceed max_selected");
+    if (a.max_selected > 0x7fffffffu) return fail(QVP_ERR_UNSUPPORTED, "lists of more than 2^31 - 1 blocks");
     if (a.batch == 0) return QVP_OK;
     qvp_block_shape ss;
     rc = qvp_summary_shape(&sh, &ss);

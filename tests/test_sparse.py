@@ -140,6 +140,12 @@ def test_select_refuses_contexts_that_do_not_fit_a_cluster():
     assert _select(max_blocks_per_seq=blocks + 1, max_context_len=(blocks + 1) * 16) == qvp.ERR_UNSUPPORTED
 
 
+@pytest.mark.parametrize("call", [_select, _attend])
+@pytest.mark.parametrize("entries", [2**31, 2**32 - 1])
+def test_lists_past_31_bits_are_refused(call, entries):
+    assert call(max_selected=entries) == qvp.ERR_UNSUPPORTED
+
+
 @pytest.mark.parametrize("fn", ["qvp_rope_append", "qvp_summarize_blocks", "qvp_select_blocks", "qvp_decode_selected"])
 def test_null_arguments_are_refused(fn):
     assert getattr(qvp.lib, fn)(None, None) == qvp.ERR_INVALID
