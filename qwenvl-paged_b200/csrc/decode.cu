@@ -1315,15 +1315,13 @@ int make_pool_map(const void* pool, uint32_t num_blocks, const qvp_block_shape& 
     if (encode == nullptr) return fail(QVP_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
     const uint32_t D = shape.head_dim;
     const uint32_t H = shape.num_kv_heads;
-    const cuuint64_t elem = shape.bytes_per_element;
     cuuint64_t dims[4] = {half, static_cast<cuuint64_t>(num_blocks) * shape.num_layers * 2 * shape.tokens_per_block, H,
                           D / half};
-    cuuint64_t strides[3] = {H * D * elem, D * elem, half * elem};
+    cuuint64_t strides[3] = {static_cast<cuuint64_t>(H) * D * 2, static_cast<cuuint64_t>(D) * 2, half * 2};
     cuuint32_t box[4] = {half, rows, hh, halves};
     cuuint32_t estr[4] = {1, 1, 1, 1};
-    CUresult r = encode(map, elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                        const_cast<void*>(pool), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        half * elem == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+    CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pool), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, half == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(QVP_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", int(r));
     return QVP_OK;

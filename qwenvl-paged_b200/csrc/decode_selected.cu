@@ -374,7 +374,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
                 if (static_cast<uint32_t>(blk[k]) >= nblk || static_cast<uint32_t>(frame[k]) >= p.num_blocks) {
                     record_error(p.err, kErrBadBlockId);
                 } else {
-                    left[k] = ctx - static_cast<int>(static_cast<uint32_t>(blk[k]) * p.T + first);
+                    const uint32_t at = static_cast<uint32_t>(blk[k]) * p.T + first;  // may pass 2^31
+                    left[k] = at < static_cast<uint32_t>(ctx) ? static_cast<int>(static_cast<uint32_t>(ctx) - at) : 0;
                     krow[k] = static_cast<int>(((static_cast<uint32_t>(frame[k]) * p.num_layers + p.layer) * 2) * p.T +
                                                first);
                 }

@@ -91,8 +91,7 @@ int encode_pool_map_box(const void* pool, uint32_t num_blocks, const qvp_block_s
                         uint32_t rows, uint32_t halves, CUtensorMap_st* map);
 // Encodes that view for blocks of any tokens_per_block T (token row of block
 // b, layer l, stream s, slot t is ((b*L + l)*2 + s)*T + t), with head_dim in
-// pieces of `half` elements, 128 or 64 bytes, swizzled over as many; either
-// element type.
+// pieces of `half` elements, 64 or 32, swizzled over their bytes.
 int make_pool_map(const void* pool, uint32_t num_blocks, const qvp_block_shape& shape, uint32_t hh, uint32_t rows,
                   uint32_t halves, CUtensorMap_st* map, uint32_t half = 64);
 

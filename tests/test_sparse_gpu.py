@@ -904,3 +904,49 @@ def test_offsets_past_32_bits():
     near_attention(d, out, q, want)
     del c, tail
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype,D,T", [("bf16", 64, 48), ("bf16", 128, 256), ("f32", 64, 48), ("f32", 80, 256)])
+def test_the_longest_context(dtype, D, T):
+    """2^31 - 1 tokens: the last block's slots end past 31 bits."""
+    torch = _torch()
+    longest = 2**31 - 1
+    last = (longest - 1) // T
+    c = Cache(36, [6 * T], dtype=dtype, hkv=1, D=D, T=T, spare=0)
+    k, v = c.make((1, 5, 1, D)), c.make((1, 5, 1, D))
+    c.pitch, c.ctx = last + 1, np.array([longest], dtype=np.int32)
+    c.ctx_d.fill_(longest)
+    c.tables_d = torch.full((1, c.pitch), -1, dtype=torch.int32, device="cuda")
+    c.tables_d[0, 0], c.tables_d[0, last - 1], c.tables_d[0, last] = 5, 1, 2
+    new = torch.tensor([5], dtype=torch.int32, device="cuda")
+    freq = torch.tensor([2.0**-k for k in range(16)], device="cuda")  # exact angles
+    before = c.pool64()
+    args = qvp.rope_append_args(**c.common(), **c.at_pool(), **c.at_summary(), num_query_heads=0, max_query_len=5,
+                                query_lens=new.data_ptr(), key=k.data_ptr(), value=v.data_ptr(), rotary_dim=32,
+                                inv_freq=freq.data_ptr())
+    assert qvp.rope_append(args, _stream()) == qvp.OK, qvp.last_error()
+    assert c.errors() == 0
+    after, k64, v64 = c.pool64(), k.double().cpu().numpy()[0, :, 0], v.double().cpu().numpy()[0, :, 0]
+    want = before.copy()
+    filled = longest - last * T
+    for t in range(5):
+        at = longest - 5 + t
+        x, y = k64[t, :16].copy(), k64[t, 16:32].copy()
+        angle = np.array([math.fmod(at * 2.0**-j, 2 * math.pi) for j in range(16)])
+        row = k64[t].copy()
+        row[:16], row[16:32] = x * np.cos(angle) - y * np.sin(angle), y * np.cos(angle) + x * np.sin(angle)
+        block, slot = (2, at - last * T) if at >= last * T else (1, at - (last - 1) * T)
+        want[block, 0, 0, slot, 0], want[block, 0, 1, slot, 0] = row, v64[t]
+    # the angle in turns is a 64-bit product below 2^29: off by 2^-25 of a turn, 2^-22 of an element's pair
+    size = np.zeros_like(want)
+    size[..., :16] = size[..., 16:32] = np.abs(want[..., :16]) + np.abs(want[..., 16:32])
+    assert (np.abs(after - want) <= STEP[dtype] * np.abs(want) + 2.0**-19 * size).all()
+    assert np.array_equal(c.summary64()[2, 0], S.summary_of(after, 2, 0, filled))
+    lists = np.array([[[0, last - 1, last]]], dtype=np.int32)
+    q = c.make((1, 4, D))
+    args, out = c.attend_args(q, torch.from_numpy(lists).cuda())
+    assert qvp.decode_selected(args, _stream()) == qvp.OK, qvp.last_error()
+    assert c.errors() == 0
+    # the same blocks as a short context
+    c.ctx, c.tables = np.array([2 * T + filled]), np.array([[5, 1, 2]])
+    near_attention(c, out, q, np.array([[[0, 1, 2]]], dtype=np.int32))
