@@ -17,7 +17,8 @@
 // A cluster of CTAs serves one (sequence, kv head): each scores its part of
 // the blocks into shared memory, and they agree on the border of the best
 // ones through distributed shared memory, so there is no workspace and no
-// second kernel. The border is found by value: the scores' range is cut into
+// second kernel. Where they are few, one CTA of the cluster gets all scores and
+// chooses alone: one barrier in place of six. The border is found by value: the scores' range is cut into
 // equal bins, the bin that holds the border is counted out, and its few
 // members are ranked exactly (value first, lower block on a tie). A bin with
 // more members than that is cut again over its own range.
@@ -36,6 +37,7 @@ constexpr int kSelWarps = kSelThreads / 32;
 constexpr uint32_t kSelBins = 512;
 constexpr uint32_t kSelBorder = kSelThreads;      // border members ranked in one go, one per thread
 constexpr uint32_t kSelMaxCluster = 8;
+constexpr uint32_t kSelMaxGather = 2048;          // blocks whose scores one CTA of a cluster gathers
 constexpr uint32_t kSelMaxChunk = 14336;          // blocks one CTA can hold: 13 bytes each of 200 KiB
 
 // States of a block during the search.
@@ -57,6 +59,7 @@ struct SelectParams {
     uint32_t keep, sink, recent;
     uint32_t cluster;
     uint32_t chunk;  // scores a CTA has room for
+    bool gather;     // the first CTA of a cluster gets all scores and chooses
 };
 
 struct SelectShared {
@@ -71,6 +74,7 @@ struct SelectShared {
     float key_lo, key_hi, top;        // the same of the keys; largest sum of a score's terms without their signs
     float warp_key_lo[kSelWarps], warp_key_hi[kSelWarps], warp_top[kSelWarps];
     uint32_t warp_sum[kSelWarps];
+    float every_top[kSelMaxCluster * kSelWarps];  // of the warps of all CTAs
     uint32_t border_count;
     uint32_t open_count;              // this CTA's open blocks
     uint32_t taken;                   // this CTA's blocks that are taken for sure
@@ -235,7 +239,8 @@ __device__ __forceinline__ void find_border(const uint32_t* total, uint32_t left
     }
 }
 
-// Takes the `need` best of the cluster's blocks (there are more), by value
+// Takes the `need` best of the cluster's blocks (there are more; `cluster` is 1
+// where this CTA has all scores), by value
 // and, on a tie, the lower block; blocks of a lower rank are lower. key_lo and
 // key_hi: the range of this thread's keys. The keys are part.score in 32 bits
 // where error_scale is 0, else scores that are off by less than error_scale
@@ -247,9 +252,9 @@ __device__ __forceinline__ void find_border(const uint32_t* total, uint32_t left
 // The first cut is by keys. Where it leaves more than kSelBorder blocks, 64-bit
 // cuts follow.
 template <typename T>
-__device__ uint32_t take_best(const SelectParams& p, const SelectPart& part, uint32_t need, float key_lo, float key_hi,
-                              float top, double error_scale, SelectShared& s) {
-    const uint32_t cluster = p.cluster, rank = part.rank, n = part.n;
+__device__ uint32_t take_best(const SelectParams& p, const SelectPart& part, uint32_t cluster, uint32_t need,
+                              float key_lo, float key_hi, float top, double error_scale, SelectShared& s) {
+    const uint32_t rank = part.rank, n = part.n;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double* const score = part.score;
     uint8_t* const state = part.state;
@@ -514,6 +519,12 @@ __device__ uint32_t take_best(const SelectParams& p, const SelectPart& part, uin
     return at;
 }
 
+// Where scores go to another CTA: it has started, its memory can be written.
+template <bool GATHER>
+__device__ __forceinline__ void wait_for_gatherer() {
+    if constexpr (GATHER) cg::this_cluster().barrier_wait();
+}
+
 // Sums over the query heads of the group: [down D | up D]. A thread's first
 // kAhead heads of its first dimension are loaded by `load`, so that other loads
 // can be issued before `store` needs them.
@@ -688,7 +699,7 @@ __device__ __forceinline__ void score_vectors(const SelectParams& p, const Selec
 // That sum is a product as well: the sizes of the weights, in a fourth column
 // of B, by the sizes of the row; its largest is `top` (infinite or NaN where a
 // row or a weight is, or is more than 32 bits hold). Returns the factor.
-template <int LOADS>
+template <int LOADS, bool GATHER>
 __device__ __forceinline__ double score_tiles(const SelectParams& p, const SelectPart& part, uint32_t b, double* weight,
                                               __nv_bfloat16* terms, float& lo, float& hi, float& top) {
     using T = __nv_bfloat16;
@@ -731,6 +742,7 @@ __device__ __forceinline__ double score_tiles(const SelectParams& p, const Selec
     __syncthreads();
     split_weights<kPitch>(p, weight, terms);
     __syncthreads();
+    wait_for_gatherer<GATHER>();
     const T* columns = terms + row * kPitch + col * 8;
 #pragma unroll 1
     for (bool first = true; base < n; base += kStride, first = false) {
@@ -779,34 +791,37 @@ template <int LOADS>
 struct ByTile {};
 
 // Scores of a part, its weights made on the way; returns their error factor.
-template <typename T>
+template <typename T, bool GATHER>
 __device__ __forceinline__ double score_part(ByElement, const SelectParams& p, const SelectPart& part, uint32_t b,
                                              double* weight, float& lo, float& hi, float&) {
     Weights<T> weights;
     weights.load(p, b, part.head);
     weights.store(p, weight);
     __syncthreads();
+    wait_for_gatherer<GATHER>();
     score_each<T>(p, part, lo, hi);
     return 0.0;
 }
-template <typename T, int LANES, int VECS>
+template <typename T, bool GATHER, int LANES, int VECS>
 __device__ __forceinline__ double score_part(ByVector<LANES, VECS>, const SelectParams& p, const SelectPart& part,
                                              uint32_t b, double* weight, float& lo, float& hi, float&) {
     Weights<T> weights;
     weights.load(p, b, part.head);
     weights.store(p, weight);
     __syncthreads();
+    wait_for_gatherer<GATHER>();
     score_vectors<T, LANES, VECS>(p, part, lo, hi);
     return 0.0;
 }
-template <typename T, int LOADS>
+template <typename T, bool GATHER, int LOADS>
 __device__ __forceinline__ double score_part(ByTile<LOADS>, const SelectParams& p, const SelectPart& part, uint32_t b,
                                              double* weight, float& lo, float& hi, float& top) {
     __shared__ __align__(16) __nv_bfloat16 terms[4 * (32 * LOADS + 8)];
-    return score_tiles<LOADS>(p, part, b, weight, terms, lo, hi, top);
+    return score_tiles<LOADS, GATHER>(p, part, b, weight, terms, lo, hi, top);
 }
 
-template <typename T, typename How>
+// GATHER: one CTA of the cluster gets all scores and chooses.
+template <typename T, typename How, bool GATHER>
 __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectParams p) {
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ SelectShared s;
@@ -815,9 +830,10 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectPara
     float* key = reinterpret_cast<float*>(score + p.chunk);
     uint8_t* state = reinterpret_cast<uint8_t*>(key + p.chunk);
 
+    const uint32_t cluster = p.cluster;
+    if constexpr (GATHER) cg::this_cluster().barrier_arrive();
     wait_for_previous_kernel();
     allow_next_kernel();
-    const uint32_t cluster = p.cluster;
     const uint32_t rank = blockIdx.x % cluster;
     const uint32_t seg = blockIdx.x / cluster;
     const uint32_t b = seg / p.hkv, head = seg % p.hkv;
@@ -825,31 +841,55 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectPara
     const int ctx = p.ctx[b];
     const bool bad = ctx < 0 || static_cast<uint32_t>(ctx) > p.max_ctx;
     const uint32_t blocks = bad ? 0u : (static_cast<uint32_t>(ctx) + p.T - 1) / p.T;
-    if (blocks <= p.keep) {  // the whole cluster
+    const uint32_t need = p.keep - p.sink - p.recent;
+    if (blocks <= p.keep) {
         if (bad && rank == 0 && threadIdx.x == 0) record_error(p.err, kErrBadContext);
         for (uint32_t i = rank * kSelThreads + threadIdx.x; i < p.keep; i += cluster * kSelThreads)
             out[i] = i < blocks ? static_cast<int32_t>(i) : -1;
+    } else {
+        if (rank == 0)
+            for (uint32_t i = threadIdx.x; i < p.sink; i += kSelThreads) out[i] = static_cast<int32_t>(i);
+        if (rank == cluster - 1)
+            for (uint32_t i = threadIdx.x; i < p.recent; i += kSelThreads)
+                out[p.keep - p.recent + i] = static_cast<int32_t>(blocks - p.recent + i);
+    }
+    if (blocks <= p.keep || need == 0) {  // the whole cluster
+        if constexpr (GATHER) cg::this_cluster().barrier_wait();
         return;
     }
     // blocks between sink and recent, this CTA's part of them
-    const uint32_t end = blocks - p.recent;
-    const uint32_t part = (end - p.sink + cluster - 1) / cluster;
-    const uint32_t first = min(p.sink + rank * part, end);
-    const uint32_t n = min(part, end - first);
-    const uint32_t need = p.keep - p.sink - p.recent;
-    if (rank == 0)
-        for (uint32_t i = threadIdx.x; i < p.sink; i += kSelThreads) out[i] = static_cast<int32_t>(i);
-    if (rank == cluster - 1)
-        for (uint32_t i = threadIdx.x; i < p.recent; i += kSelThreads)
-            out[p.keep - p.recent + i] = static_cast<int32_t>(end + i);
-    if (need == 0) return;  // the whole cluster
-
-    const SelectPart work = {p.tables + static_cast<size_t>(b) * p.pitch + first, weight, key, score, state, first, n, head,
-                             rank};
+    const uint32_t open = blocks - p.recent - p.sink;
+    const int32_t* table = p.tables + static_cast<size_t>(b) * p.pitch + p.sink;
+    const uint32_t share = (open + cluster - 1) / cluster, from = min(rank * share, open);
+    SelectPart work = {table + from, weight, key, score, state, p.sink + from, min(share, open - from), head, rank};
+    if constexpr (GATHER) {
+        work.key = of_rank(key, cluster, 0) + from;
+        work.score = of_rank(score, cluster, 0) + from;
+    }
     float lo = INFINITY, hi = -INFINITY, top = 0.f;
-    const double error_scale = score_part<T>(How{}, p, work, b, weight, lo, hi, top);
-    __syncthreads();
-    const uint32_t before = take_best<T>(p, work, need, lo, hi, top, error_scale, s);
+    const double error_scale = score_part<T, GATHER>(How{}, p, work, b, weight, lo, hi, top);
+    if constexpr (GATHER) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if ((threadIdx.x & 31) == 0)
+            *of_rank(&s.every_top[rank * kSelWarps + (threadIdx.x >> 5)], cluster, 0) = top;
+        cg::this_cluster().sync();
+        if (rank != 0) return;
+        work = {table, weight, key, score, state, p.sink, open, head, 0};
+        lo = INFINITY;
+        hi = -INFINITY;
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < open; i += kSelThreads) {
+            lo = fminf(lo, key[i]);
+            hi = fmaxf(hi, key[i]);
+        }
+        top = s.every_top[threadIdx.x % (cluster * kSelWarps)];
+    } else {
+        __syncthreads();
+    }
+    const uint32_t joint = GATHER ? 1 : cluster;  // CTAs that choose together
+    const uint32_t n = work.n;
+    const uint32_t before = take_best<T>(p, work, joint, need, lo, hi, top, error_scale, s);
 
     // ascending list: what the ranks took, in rank order, a run of blocks per thread
     const uint32_t per = (n + kSelThreads - 1) / kSelThreads;
@@ -859,20 +899,26 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectPara
     uint32_t all;
     int32_t* to = out + p.sink + before + cta_scan(mine, all, s);
     for (uint32_t i = run; i < stop; ++i)
-        if (state[i] == kTaken) *to++ = static_cast<int32_t>(first + i);
+        if (state[i] == kTaken) *to++ = static_cast<int32_t>(work.first + i);
     // no CTA leaves while another may read its shared memory
-    if (cluster > 1) cg::this_cluster().barrier_wait();
+    if (joint > 1) cg::this_cluster().barrier_wait();
 }
 
-template <typename T, typename How>
-int launch_select_t(How, const SelectParams& p, uint32_t segments, size_t smem, cudaStream_t st) {
+template <typename T, typename How, bool GATHER>
+int launch_select_g(const SelectParams& p, uint32_t segments, size_t smem, cudaStream_t st) {
     static std::atomic<std::uint64_t> attr_done{0};
-    auto kern = select_kernel<T, How>;
+    auto kern = select_kernel<T, How, GATHER>;
     const int rc = set_smem_limit_once(attr_done, reinterpret_cast<const void*>(kern), 200 * 1024,
                                        "cudaFuncSetAttribute(select_blocks)");
     if (rc != QVP_OK) return rc;
     return launch_dependent("launch select_blocks", kern, dim3(segments * p.cluster), kSelThreads, smem, p.cluster, st,
                             p);
+}
+
+template <typename T, typename How>
+int launch_select_t(How, const SelectParams& p, uint32_t segments, size_t smem, cudaStream_t st) {
+    return p.gather ? launch_select_g<T, How, true>(p, segments, smem, st)
+                    : launch_select_g<T, How, false>(p, segments, smem, st);
 }
 
 template <typename T>
@@ -965,7 +1011,10 @@ extern "C" int qvp_select_blocks(const qvp_select_args* args, qvp_stream_t strea
     while (p.cluster < kSelMaxCluster && (ceil_div(scored, p.cluster) > kSelMaxChunk ||
                                           (segments * p.cluster <= sms && scored / p.cluster > 64)))
         p.cluster *= 2;
-    p.chunk = static_cast<uint32_t>(round_up(ceil_div(scored, p.cluster), 16));
+    // One row of 1024 blocks: 9.9 us gathered, 11.2 not; 2048: 12.1 and 12.7;
+    // 4096: 16.6 and 15.1.
+    p.gather = p.cluster > 1 && scored <= kSelMaxGather;
+    p.chunk = static_cast<uint32_t>(round_up(p.gather ? scored : ceil_div(scored, p.cluster), 16));
     if (p.chunk > kSelMaxChunk)
         return fail(QVP_ERR_UNSUPPORTED, "contexts of more than %u blocks", kSelMaxChunk * kSelMaxCluster);
     if (segments * p.cluster > 0x7fffffffu) return fail(QVP_ERR_UNSUPPORTED, "more than 2^31 sequences and heads");
