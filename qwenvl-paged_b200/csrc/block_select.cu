@@ -43,6 +43,10 @@ constexpr uint32_t kSelMaxChunk = 14336;          // blocks one CTA can hold: 13
 // States of a block during the search.
 enum : uint8_t { kOpen = 0, kTaken = 1, kDropped = 2 };
 
+// Who chooses: a CTA its own blocks, the CTAs of a cluster together, or the
+// first of them, which gets all scores.
+enum Chooser { kAlone, kJointly, kFirst };
+
 struct SelectParams {
     const uint8_t* summary;
     size_t summary_stride;
@@ -59,7 +63,7 @@ struct SelectParams {
     uint32_t keep, sink, recent;
     uint32_t cluster;
     uint32_t chunk;  // scores a CTA has room for
-    bool gather;     // the first CTA of a cluster gets all scores and chooses
+    Chooser who;
 };
 
 struct SelectShared {
@@ -520,9 +524,9 @@ __device__ uint32_t take_best(const SelectParams& p, const SelectPart& part, uin
 }
 
 // Where scores go to another CTA: it has started, its memory can be written.
-template <bool GATHER>
-__device__ __forceinline__ void wait_for_gatherer() {
-    if constexpr (GATHER) cg::this_cluster().barrier_wait();
+template <Chooser WHO>
+__device__ __forceinline__ void wait_for_chooser() {
+    if constexpr (WHO == kFirst) cg::this_cluster().barrier_wait();
 }
 
 // Sums over the query heads of the group: [down D | up D]. A thread's first
@@ -699,7 +703,7 @@ __device__ __forceinline__ void score_vectors(const SelectParams& p, const Selec
 // That sum is a product as well: the sizes of the weights, in a fourth column
 // of B, by the sizes of the row; its largest is `top` (infinite or NaN where a
 // row or a weight is, or is more than 32 bits hold). Returns the factor.
-template <int LOADS, bool GATHER>
+template <int LOADS, Chooser WHO>
 __device__ __forceinline__ double score_tiles(const SelectParams& p, const SelectPart& part, uint32_t b, double* weight,
                                               __nv_bfloat16* terms, float& lo, float& hi, float& top) {
     using T = __nv_bfloat16;
@@ -742,7 +746,7 @@ __device__ __forceinline__ double score_tiles(const SelectParams& p, const Selec
     __syncthreads();
     split_weights<kPitch>(p, weight, terms);
     __syncthreads();
-    wait_for_gatherer<GATHER>();
+    wait_for_chooser<WHO>();
     const T* columns = terms + row * kPitch + col * 8;
 #pragma unroll 1
     for (bool first = true; base < n; base += kStride, first = false) {
@@ -791,37 +795,36 @@ template <int LOADS>
 struct ByTile {};
 
 // Scores of a part, its weights made on the way; returns their error factor.
-template <typename T, bool GATHER>
+template <typename T, Chooser WHO>
 __device__ __forceinline__ double score_part(ByElement, const SelectParams& p, const SelectPart& part, uint32_t b,
                                              double* weight, float& lo, float& hi, float&) {
     Weights<T> weights;
     weights.load(p, b, part.head);
     weights.store(p, weight);
     __syncthreads();
-    wait_for_gatherer<GATHER>();
+    wait_for_chooser<WHO>();
     score_each<T>(p, part, lo, hi);
     return 0.0;
 }
-template <typename T, bool GATHER, int LANES, int VECS>
+template <typename T, Chooser WHO, int LANES, int VECS>
 __device__ __forceinline__ double score_part(ByVector<LANES, VECS>, const SelectParams& p, const SelectPart& part,
                                              uint32_t b, double* weight, float& lo, float& hi, float&) {
     Weights<T> weights;
     weights.load(p, b, part.head);
     weights.store(p, weight);
     __syncthreads();
-    wait_for_gatherer<GATHER>();
+    wait_for_chooser<WHO>();
     score_vectors<T, LANES, VECS>(p, part, lo, hi);
     return 0.0;
 }
-template <typename T, bool GATHER, int LOADS>
+template <typename T, Chooser WHO, int LOADS>
 __device__ __forceinline__ double score_part(ByTile<LOADS>, const SelectParams& p, const SelectPart& part, uint32_t b,
                                              double* weight, float& lo, float& hi, float& top) {
     __shared__ __align__(16) __nv_bfloat16 terms[4 * (32 * LOADS + 8)];
-    return score_tiles<LOADS, GATHER>(p, part, b, weight, terms, lo, hi, top);
+    return score_tiles<LOADS, WHO>(p, part, b, weight, terms, lo, hi, top);
 }
 
-// GATHER: one CTA of the cluster gets all scores and chooses.
-template <typename T, typename How, bool GATHER>
+template <typename T, typename How, Chooser WHO>
 __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectParams p) {
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ SelectShared s;
@@ -830,8 +833,8 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectPara
     float* key = reinterpret_cast<float*>(score + p.chunk);
     uint8_t* state = reinterpret_cast<uint8_t*>(key + p.chunk);
 
-    const uint32_t cluster = p.cluster;
-    if constexpr (GATHER) cg::this_cluster().barrier_arrive();
+    const uint32_t cluster = WHO == kAlone ? 1 : p.cluster;
+    if constexpr (WHO == kFirst) cg::this_cluster().barrier_arrive();
     wait_for_previous_kernel();
     allow_next_kernel();
     const uint32_t rank = blockIdx.x % cluster;
@@ -854,7 +857,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectPara
                 out[p.keep - p.recent + i] = static_cast<int32_t>(blocks - p.recent + i);
     }
     if (blocks <= p.keep || need == 0) {  // the whole cluster
-        if constexpr (GATHER) cg::this_cluster().barrier_wait();
+        if constexpr (WHO == kFirst) cg::this_cluster().barrier_wait();
         return;
     }
     // blocks between sink and recent, this CTA's part of them
@@ -862,13 +865,13 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectPara
     const int32_t* table = p.tables + static_cast<size_t>(b) * p.pitch + p.sink;
     const uint32_t share = (open + cluster - 1) / cluster, from = min(rank * share, open);
     SelectPart work = {table + from, weight, key, score, state, p.sink + from, min(share, open - from), head, rank};
-    if constexpr (GATHER) {
+    if constexpr (WHO == kFirst) {
         work.key = of_rank(key, cluster, 0) + from;
         work.score = of_rank(score, cluster, 0) + from;
     }
     float lo = INFINITY, hi = -INFINITY, top = 0.f;
-    const double error_scale = score_part<T, GATHER>(How{}, p, work, b, weight, lo, hi, top);
-    if constexpr (GATHER) {
+    const double error_scale = score_part<T, WHO>(How{}, p, work, b, weight, lo, hi, top);
+    if constexpr (WHO == kFirst) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
         if ((threadIdx.x & 31) == 0)
@@ -887,7 +890,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectPara
     } else {
         __syncthreads();
     }
-    const uint32_t joint = GATHER ? 1 : cluster;  // CTAs that choose together
+    const uint32_t joint = WHO == kJointly ? cluster : 1;  // CTAs that choose together
     const uint32_t n = work.n;
     const uint32_t before = take_best<T>(p, work, joint, need, lo, hi, top, error_scale, s);
 
@@ -904,10 +907,10 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectPara
     if (joint > 1) cg::this_cluster().barrier_wait();
 }
 
-template <typename T, typename How, bool GATHER>
+template <typename T, typename How, Chooser WHO>
 int launch_select_g(const SelectParams& p, uint32_t segments, size_t smem, cudaStream_t st) {
     static std::atomic<std::uint64_t> attr_done{0};
-    auto kern = select_kernel<T, How, GATHER>;
+    auto kern = select_kernel<T, How, WHO>;
     const int rc = set_smem_limit_once(attr_done, reinterpret_cast<const void*>(kern), 200 * 1024,
                                        "cudaFuncSetAttribute(select_blocks)");
     if (rc != QVP_OK) return rc;
@@ -917,8 +920,9 @@ int launch_select_g(const SelectParams& p, uint32_t segments, size_t smem, cudaS
 
 template <typename T, typename How>
 int launch_select_t(How, const SelectParams& p, uint32_t segments, size_t smem, cudaStream_t st) {
-    return p.gather ? launch_select_g<T, How, true>(p, segments, smem, st)
-                    : launch_select_g<T, How, false>(p, segments, smem, st);
+    return p.who == kAlone     ? launch_select_g<T, How, kAlone>(p, segments, smem, st)
+           : p.who == kJointly ? launch_select_g<T, How, kJointly>(p, segments, smem, st)
+                               : launch_select_g<T, How, kFirst>(p, segments, smem, st);
 }
 
 template <typename T>
@@ -1011,10 +1015,10 @@ extern "C" int qvp_select_blocks(const qvp_select_args* args, qvp_stream_t strea
     while (p.cluster < kSelMaxCluster && (ceil_div(scored, p.cluster) > kSelMaxChunk ||
                                           (segments * p.cluster <= sms && scored / p.cluster > 64)))
         p.cluster *= 2;
-    // One row of 1024 blocks: 9.9 us gathered, 11.2 not; 2048: 12.1 and 12.7;
-    // 4096: 16.6 and 15.1.
-    p.gather = p.cluster > 1 && scored <= kSelMaxGather;
-    p.chunk = static_cast<uint32_t>(round_up(p.gather ? scored : ceil_div(scored, p.cluster), 16));
+    // Four rows of 1024 blocks: 9.4 us if the first CTA chooses, 11.2 if all
+    // do; of 2048: 11.4 and 12.7; of 4096: 15.1 and 14.9.
+    p.who = p.cluster == 1 ? kAlone : scored > kSelMaxGather ? kJointly : kFirst;
+    p.chunk = static_cast<uint32_t>(round_up(p.who == kFirst ? scored : ceil_div(scored, p.cluster), 16));
     if (p.chunk > kSelMaxChunk)
         return fail(QVP_ERR_UNSUPPORTED, "contexts of more than %u blocks", kSelMaxChunk * kSelMaxCluster);
     if (segments * p.cluster > 0x7fffffffu) return fail(QVP_ERR_UNSUPPORTED, "more than 2^31 sequences and heads");
