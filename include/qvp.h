@@ -344,7 +344,9 @@ QVP_API int qvp_kv_append(void* pool, size_t block_stride, uint32_t num_blocks,
  * Lengths, tables and lists are read on the device only: entries that are
  * wrong set bits of *error_word (1: an id outside the pool or a list entry
  * past the context; 4: a length out of range) and are skipped, so no access
- * leaves the pool. The block id -1 past a context is never read. No
+ * leaves the pool. QVP_ERR_UNSUPPORTED answers shapes past the kernels'
+ * counters: head_dim above 256, a batch above 65535, blocks of more than 65536
+ * tokens or 2^31 - 1 elements of K in a layer. The block id -1 past a context is never read. No
  * counterpart in the reference (it attends every token).
  * ------------------------------------------------------------------------- */
 
@@ -461,7 +463,8 @@ QVP_API int qvp_summarize_blocks(const qvp_summarize_args* args, qvp_stream_t st
  * on how the work is split. A score that is NaN (summaries or queries that
  * hold NaN, or infinities against zeros) counts as +infinity. The summaries
  * of blocks inside sink and recent are not read. Attention with a negative
- * scale would need the opposite score.
+ * scale would need the opposite score. max_context_len may span 114,688 blocks
+ * between sink and recent; more are refused with QVP_ERR_UNSUPPORTED.
  */
 typedef struct qvp_select_args {
     const void* summary;
@@ -495,7 +498,11 @@ QVP_API int qvp_select_blocks(const qvp_select_args* args, qvp_stream_t stream);
  * leaves no token (every entry < 0, or context_lens[b] = 0) gives zeros.
  * Entries past the context set error bit 1 and are skipped; a context_lens
  * entry out of range sets bit 4 and leaves out[b] as it was. Outputs are
- * the same bits from call to call.
+ * the same bits from call to call. QVP_ERR_UNSUPPORTED answers lists of more
+ * than 2^31 - 1 tokens and more than 2^28 (sequence, kv head) pairs. The dense
+ * cache layout with head_dim 64, 96 or 128, bf16 and blocks of 8 or a multiple
+ * of 16 tokens, query and out 4-byte aligned, runs on the tensor cores; every
+ * other call takes a slower kernel of the same results.
  */
 typedef struct qvp_decode_selected_args {
     const void* pool;
