@@ -12,13 +12,13 @@
 // tokens of one cache block (so a block's summary belongs to one CTA) and
 // either its K and V or some of its query heads. It makes the cosines and sines
 // of its tokens once for all heads, in shared memory; then each thread goes
-// through the heads with those of its run of pairs of one token in registers.
+// through the heads with those of its run of pairs of one token in registers,
+// the next heads on their way in registers or in shared memory.
 //
 // Measured (28 + 4 + 4 heads of 128, bf16): 16 prompts of 2,048 tokens, 609 MB,
-// 120 us, 5.1 TB/s, waiting for loads (two heads of a thread are in flight); 64
-// single tokens 5.2 us. 7 ragged fp32 chunks, 11 MB: 7.1 us. With the heads in
-// flight in shared memory, a ring of four per thread, the prompts took 114 us,
-// the others 5.8 and 8.4.
+// 110.9 us, 5.5 TB/s; 64 single tokens 5.3 us. 7 ragged fp32 chunks, 11 MB: 7.9
+// us. 16 tokens at a time instead of 8 took 120 us for the prompts through
+// registers, 4 took 123.
 #include "sparse_common.cuh"
 
 namespace qvp {
@@ -26,7 +26,8 @@ namespace qvp {
 namespace {
 
 constexpr int kRopeThreads = 128;
-constexpr uint32_t kRopeTokens = 16;  // most tokens of a CTA at a time
+constexpr uint32_t kRopeTokens = 8;   // most tokens of a CTA at a time
+constexpr uint32_t kRing = 4;         // heads a thread has on their way to shared memory
 constexpr uint32_t kMaxPairs = 128;   // head_dim <= 256
 
 struct RopeParams {
@@ -150,7 +151,7 @@ __device__ __forceinline__ void rotate(Vec<T, VEC>& a, Vec<T, VEC>& b, const flo
 }
 
 // Turns (or copies) one item of heads [0, count) of a token, every step-th
-// from `first` on: rows src + h * D to dst + h * D.
+// from `first` on: rows src + h * D to dst + h * D, two of them in registers.
 template <typename T, int VEC>
 __device__ __forceinline__ void turn_heads(const T* src, T* dst, uint32_t first, uint32_t count, uint32_t step,
                                            uint32_t D, const Item<VEC>& x, const float2 (&cs)[VEC], bool interleaved) {
@@ -178,15 +179,58 @@ __device__ __forceinline__ void turn_heads(const T* src, T* dst, uint32_t first,
     }
 }
 
-// VEC elements at a time where rows and halves fall on 16-byte boundaries,
-// else one by one. grid (batch * units, 1 + groups of query heads).
+// The same with kRing heads on their way to shared memory, to vectors that only
+// this thread touches: it waits for its own copies and for no other thread.
 template <typename T, int VEC>
+struct HeadRing {
+    const T* src;
+    uint32_t first, count, step, D;
+    Item<VEC> x;
+
+    // Vectors of turn k: thread by thread, so that a warp's lie side by side.
+    static __device__ __forceinline__ Vec<T, VEC>* place(Vec<T, VEC>* ring, uint32_t k, uint32_t v) {
+        return ring + (k % kRing * 2 + v) * kRopeThreads + threadIdx.x;
+    }
+    __device__ __forceinline__ void ask_one(Vec<T, VEC>* ring, uint32_t k) const {
+        const uint32_t h = first + k * step;
+        if (h < count) {
+            const uint32_t a = smem_u32(place(ring, k, 0)), b = smem_u32(place(ring, k, 1));
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(src + h * D + x.e0) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(b), "l"(src + h * D + x.e1) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    __device__ __forceinline__ void ask(Vec<T, VEC>* ring) const {
+#pragma unroll
+        for (uint32_t k = 0; k < kRing; ++k) ask_one(ring, k);
+    }
+    __device__ __forceinline__ void run(Vec<T, VEC>* ring, T* dst, const float2 (&cs)[VEC], bool interleaved) const {
+        uint32_t k = 0;
+        for (uint32_t h = first; h < count; h += step, ++k) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+            Vec<T, VEC> u = *place(ring, k, 0), w = *place(ring, k, 1);
+            if (x.turned) rotate<T, VEC>(u, w, cs, interleaved);
+            store_vec<T, VEC>(dst + h * D + x.e0, u);
+            store_vec<T, VEC>(dst + h * D + x.e1, w);
+            ask_one(ring, k + kRing);
+        }
+    }
+};
+
+// VEC elements at a time where rows and halves fall on 16-byte boundaries,
+// else one by one. grid (batch * units, 1 + groups of query heads). RING: heads
+// on their way in shared memory, and keys and values last, so that the long
+// CTAs do not start last; else in registers, and keys and values first, whose
+// way through table and summary is the longest.
+template <typename T, int VEC, bool RING>
 __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeParams p) {
     // of pair it * VEC + j of token t at [j][t * row_items + it], rows one apart
     // from a multiple of the banks
     __shared__ float2 table[kRopeTokens * kMaxPairs + VEC];
-    // partial ranges of the token groups of K, two vectors each
-    __shared__ Vec<T, VEC> part[kRopeThreads][4];
+    // heads on their way, and at the end partial ranges of the token groups of
+    // K, two vectors each
+    __shared__ Vec<T, VEC> ring[(RING ? 2 * kRing : 4) * kRopeThreads];
+    Vec<T, VEC>(*part)[4] = reinterpret_cast<Vec<T, VEC>(*)[4]>(ring);
 
     wait_for_previous_kernel();
     allow_next_kernel();
@@ -205,7 +249,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
     const uint32_t lo = max(first, base);                                       // new positions [lo, hi)
     const uint32_t hi = min(static_cast<uint32_t>(ctx), base + p.T);
 
-    const bool kv = blockIdx.y == 0;
+    const bool kv = blockIdx.y == (RING ? gridDim.y - 1 : 0);
     uint8_t* frame = nullptr;
     int32_t id = 0;
     if (kv) {
@@ -224,7 +268,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
     const size_t row0 = static_cast<size_t>(b) * p.max_q + (lo - first);        // token row of position lo
     const uint32_t cnt = hi - lo;
     const uint32_t half = p.rotary / 2;
-    const uint32_t h0 = kv ? 0 : (blockIdx.y - 1) * p.heads_per_cta;
+    const uint32_t h0 = kv ? 0 : (RING ? blockIdx.y : blockIdx.y - 1) * p.heads_per_cta;
     const uint32_t nh = kv ? p.hkv : min(p.heads_per_cta, p.hq - h0);
     const T* src = kv ? static_cast<const T*>(p.k) + row0 * p.k_pitch
                       : static_cast<const T*>(p.q) + row0 * p.q_pitch + static_cast<size_t>(h0) * D;
@@ -249,6 +293,14 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
     }
     for (uint32_t t0 = 0; t0 < cnt; t0 += p.tokens) {
         const uint32_t some = min(p.tokens, cnt - t0);
+        auto ring_at = [&](uint32_t i) -> HeadRing<T, VEC> {
+            return {src + (t0 + i / row_items % p.tokens) * src_pitch, i / places, nh, sharers, D,
+                    Item<VEC>(i % row_items, p.rotary, p.interleaved)};
+        };
+        if constexpr (RING) {  // the angles are made while the first heads come
+            if (threadIdx.x < places * sharers && threadIdx.x / row_items % p.tokens < some)
+                ring_at(threadIdx.x).ask(ring);
+        }
         if (t0 > 0) __syncthreads();
         if (threadIdx.x < at_once * half) {
 #pragma unroll 4
@@ -267,8 +319,14 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) cs[j] = table[j * (places + 1) + t * row_items + it];
             }
-            turn_heads<T, VEC>(src + (t0 + t) * src_pitch, dst + (t0 + t) * dst_pitch, i / places, nh, sharers, D, x, cs,
-                               p.interleaved);
+            if constexpr (RING) {
+                const HeadRing<T, VEC> mine = ring_at(i);
+                if (i != threadIdx.x) mine.ask(ring);  // all its copies before have been used
+                mine.run(ring, dst + (t0 + t) * dst_pitch, cs, p.interleaved);
+            } else {
+                turn_heads<T, VEC>(src + (t0 + t) * src_pitch, dst + (t0 + t) * dst_pitch, i / places, nh, sharers, D, x,
+                                   cs, p.interleaved);
+            }
         }
     }
     if (kv) {
@@ -337,11 +395,13 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
 }
 
 template <typename T>
-int launch_rope(const RopeParams& p, bool vec, dim3 grid, cudaStream_t st) {
-    if (vec)
-        return launch_dependent("launch rope_append", rope_append_kernel<T, 16 / sizeof(T)>, grid, kRopeThreads, 0, 1,
-                                st, p);
-    return launch_dependent("launch rope_append", rope_append_kernel<T, 1>, grid, kRopeThreads, 0, 1, st, p);
+int launch_rope(const RopeParams& p, bool vec, bool ring, dim3 grid, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    const char* what = "launch rope_append";
+    if (vec && ring)
+        return launch_dependent(what, rope_append_kernel<T, V, true>, grid, kRopeThreads, 0, 1, st, p);
+    if (vec) return launch_dependent(what, rope_append_kernel<T, V, false>, grid, kRopeThreads, 0, 1, st, p);
+    return launch_dependent(what, rope_append_kernel<T, 1, false>, grid, kRopeThreads, 0, 1, st, p);
 }
 
 }  // namespace
@@ -462,5 +522,14 @@ extern "C" int qvp_rope_append(const qvp_rope_append_args* args, qvp_stream_t st
                       (aligned_to(a.query, 16) && aligned_to(a.query_out, 16) && q_pitch % V == 0)) &&
                      (a.summary == nullptr || (aligned_to(a.summary, 16) && a.summary_stride % 16 == 0));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    return a.dtype == QVP_DTYPE_F32 ? launch_rope<float>(p, vec, grid, st) : launch_rope<__nv_bfloat16>(p, vec, grid, st);
+    // Heads through shared memory where a thread has at least a ring of them and
+    // CTAs come in waves: 16 prompts of 2,048 tokens (28 + 4 + 4 heads of 128,
+    // bf16) 110.9 us, 116.2 through registers; 32 of 512: 59.3 and 65.9. Else
+    // registers: 2 prompts of 2,048 23.0 us, 26.8 through shared memory; 1,024
+    // single tokens 12.0 and 13.2.
+    const uint32_t places = p.tokens * (D / (2 * V));
+    const uint32_t sharers = places > 0 && places < kRopeThreads ? kRopeThreads / places : 1;
+    const bool ring = p.heads_per_cta >= kRing * sharers && static_cast<uint64_t>(grid.x) * grid.y > 8 * sms;
+    return a.dtype == QVP_DTYPE_F32 ? launch_rope<float>(p, vec, ring, grid, st)
+                                    : launch_rope<__nv_bfloat16>(p, vec, ring, grid, st);
 }

@@ -255,6 +255,19 @@ def test_append_long_chunks(new):
     run_append(c, new, 4, most=701)
 
 
+@pytest.mark.parametrize("dtype,hq,hkv,D,T,most", [("bf16", 16, 4, 64, 8, 200), ("bf16", 17, 1, 64, 16, 400),
+                                                   ("f32", 8, 2, 64, 16, 400), ("bf16", 12, 2, 256, 8, 200),
+                                                   ("f32", 4, 1, 256, 8, 200), ("bf16", 10, 5, 96, 16, 400)])
+@pytest.mark.parametrize("kw", [dict(), dict(fused=True, interleaved=True), dict(in_place=True, rotary=32)])
+def test_append_prompts_of_a_full_batch(dtype, hq, hkv, D, T, most, kw):
+    """Several waves of CTAs whose threads take several heads each; lengths from none to all rows."""
+    rng = np.random.default_rng(37)
+    new = rng.integers(0, most + 1, size=24)
+    new[:5] = most, 0, 1, most - 1, T
+    c = Cache(38, new + rng.integers(0, 3 * T, size=24), dtype=dtype, hkv=hkv, D=D, T=T)
+    run_append(c, new, hq, most=most, **kw)
+
+
 def test_append_cache_positions_are_the_default():
     c = Cache(5, [100, 37], hkv=2, D=64)
     run_append(c, [40, 37], 4, positions=None)
