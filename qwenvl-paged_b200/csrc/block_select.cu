@@ -18,15 +18,15 @@
 // the blocks into shared memory, and they agree on the border of the best
 // ones through distributed shared memory, so there is no workspace and no
 // second kernel. Where they are few, one CTA of the cluster gets all scores and
-// chooses alone: one barrier in place of six. The border is found by value: the scores' range is cut into
-// equal bins, the bin that holds the border is counted out, and its few
-// members are ranked exactly (value first, lower block on a tie). A bin with
-// more members than that is cut again over its own range.
+// chooses alone: one barrier in place of six. The border is found by value: the
+// scores' range is cut into equal bins, the bin that holds the border is counted
+// out, and its few members are ranked exactly (value first, lower block on a
+// tie). A bin with more members than that is cut again over its own range.
 //
 // Measured (bf16, head_dim 128, blocks of 16): 32 contexts of 32,768 tokens with
-// 8 kv heads, 128 kept, 269 MB of summaries: 52.6 us, 5.1 TB/s, of which about 7
+// 8 kv heads, 128 kept, 269 MB of summaries: 51.5 us, 5.2 TB/s, of which about 7
 // are the choice at the end of every CTA; 64 contexts of 512 to 8,192 tokens
-// with 4 kv heads, 38 MB: 16.0 us; one of 32,768 with 8: 11.5 us, a chain of
+// with 4 kv heads, 38 MB: 15.6 us; one of 32,768 with 8: 11.5 us, a chain of
 // latencies.
 #include "sparse_common.cuh"
 
@@ -609,7 +609,9 @@ __device__ __forceinline__ void score_each(const SelectParams& p, const SelectPa
 // The same with 16-byte loads: LANES lanes per block, VECS vectors a lane, and
 // UNROLL blocks of every lane group per step. A lane keeps the weights of its
 // columns in registers, and the UNROLL partial sums of a group are reduced
-// together: each exchange halves the sums a lane carries.
+// together: each exchange halves the sums a lane carries. Rows are read once,
+// first out of the cache: 64 ragged contexts with head_dim 80 take 22.4 us, with
+// plain loads 24.8; fp32 with head_dim 128 27.1 and 27.6.
 template <typename T, int LANES, int VECS>
 __device__ __forceinline__ void score_vectors(const SelectParams& p, const SelectPart& part, float& lo, float& hi) {
     constexpr int V = 16 / sizeof(T);
@@ -647,7 +649,9 @@ __device__ __forceinline__ void score_vectors(const SelectParams& p, const Selec
             const int32_t id = __shfl_sync(0xffffffffu, bad ? 0 : ids, u * kGroups + group);
 #pragma unroll
             for (int j = 0; j < VECS; ++j)
-                if (live[j]) x[u][j] = load_vec<T, V>(rows + static_cast<size_t>(id) * stride + j * LANES * V);
+                if (live[j])
+                    *reinterpret_cast<uint4*>(&x[u][j]) = __ldcs(
+                        reinterpret_cast<const uint4*>(rows + static_cast<size_t>(id) * stride + j * LANES * V));
         }
         double s[UNROLL];
 #pragma unroll
@@ -738,10 +742,12 @@ __device__ __forceinline__ double score_tiles(const SelectParams& p, const Selec
         if (bad0 || bad1) record_error(p.err, kErrBadBlockId);
         const T* at0 = rows + static_cast<size_t>(bad0 ? 0 : id0) * stride;
         const T* at1 = rows + static_cast<size_t>(bad1 ? 0 : id1) * stride;
+        // read once, first out: 51.5 us where plain loads took 52.5 (32 contexts of
+        // 32,768 tokens)
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
-            x[j] = *reinterpret_cast<const uint4*>(at0 + j * 32);
-            y[j] = *reinterpret_cast<const uint4*>(at1 + j * 32);
+            x[j] = __ldcs(reinterpret_cast<const uint4*>(at0 + j * 32));
+            y[j] = __ldcs(reinterpret_cast<const uint4*>(at1 + j * 32));
         }
         id0 = id_of(base + kStride + row);
         id1 = id_of(base + kStride + row + 8);
@@ -1014,7 +1020,7 @@ extern "C" int qvp_select_blocks(const qvp_select_args* args, qvp_stream_t strea
     const uint32_t scored = blocks > a.max_selected ? blocks - a.sink_blocks - a.recent_blocks : 0;
     const uint64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
     // Two CTAs are resident per SM: share a list of scores while the whole grid
-    // still is (256 rows of 2048 blocks: 52.6 us with one CTA a row, 63.2 with
+    // still is (256 rows of 2048 blocks: 51.5 us with one CTA a row, 63.2 with
     // two; 8 rows: 23.2 with one, 11.4 with eight), and as far as they have to
     // to hold it.
     p.cluster = 1;

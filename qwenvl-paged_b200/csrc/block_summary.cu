@@ -1,16 +1,17 @@
 // Block summaries: per-channel minimum and maximum of a block's K, the input
 // of the block score. Bound by HBM: K is read once (a summary is 2 /
 // tokens_per_block of it), so a thread owns one 16-byte column of a block's
-// token rows and has the loads of many slots in flight. Measured: 64 contexts
-// of 512 to 8,192 tokens (4 heads of 128, bf16, 312 MB) 52.7 us, 5.9 TB/s; 4
-// short fp32 ones 3.4 us.
+// token rows and has the loads of four slots in flight. Measured: 64 contexts
+// of 512 to 8,192 tokens (4 heads of 128, 312 MB in bf16) 51.9 us, 6.0 TB/s, in
+// fp32 101 us, 6.7 TB/s; 4 short fp32 ones 2.7 us. Eight slots and 256 threads:
+// 52.6, 107.6 and 3.4.
 #include "sparse_common.cuh"
 
 namespace qvp {
 
 namespace {
 
-constexpr int kSummaryThreads = 256;
+constexpr int kSummaryThreads = 128;
 
 struct SummaryParams {
     const uint8_t* pool;
@@ -59,7 +60,7 @@ __global__ void __launch_bounds__(kSummaryThreads) summarize_kernel(const Summar
                  static_cast<size_t>(p.layer) * 2 * p.T * row + e;
     Vec<T, VEC> lo, hi;
     start_range(lo, hi);
-#pragma unroll 8
+#pragma unroll 4
     for (uint32_t s = 0; s < filled; ++s) {
         const Vec<T, VEC> x = load_vec<T, VEC>(k + static_cast<size_t>(s) * row);
         widen(lo, hi, x, x);
