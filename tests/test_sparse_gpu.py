@@ -479,6 +479,62 @@ def test_select_ranks_nan_and_infinities(batch):
     assert (got == [0, 1, 2, 3, 4, 399]).all()
 
 
+@pytest.mark.parametrize("dtype,D,pad", [("f32", 128, 0), ("f32", 33, 0), ("f32", 200, 0), ("bf16", 80, 0),
+                                         ("bf16", 96, 0), ("bf16", 64, 1), ("bf16", 128, 8), ("bf16", 256, 0)])
+@pytest.mark.parametrize("blocks,batch", [(300, 3), (1100, 2), (2048 + 3, 1), (2048 + 4, 1), (4100, 1)])
+def test_select_where_ctas_share_a_context(dtype, D, pad, blocks, batch):
+    """One context next to short ones and an empty one, on either side of what a CTA gathers."""
+    ctx = [blocks * 16 - 5] + [64 * 16, 0][:batch - 1]
+    c = Cache(20, ctx, dtype=dtype, layers=2, layer=1, hkv=2, D=D, pad=pad)
+    sort_summaries(c)
+    q = c.make((batch, 8, D))
+    for keep, sink, recent in ((40, 1, 2), (3, 1, 2), (64, 0, 0)):  # the second leaves nothing to choose
+        run_select(c, q, keep, sink, recent)
+
+
+@pytest.mark.parametrize("kind", ["equal", "few", "steep", "zeros", "outlier", "tiny", "close", "huge"])
+@pytest.mark.parametrize("batch,blocks", [(1, 1500), (1, 2600), (64, 300)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_select_bf16_where_scores_tie_or_crowd(kind, batch, blocks, D):
+    """The 32-bit scores leave more blocks open than one pass can rank, or none that it may trust."""
+    torch = _torch()
+    c = Cache(21, [blocks * 16] * batch, hkv=1, D=D)
+    v = c.summary[:, :c.sum_n].view(c.blocks, 2, D)
+    rng = np.random.default_rng(22)
+    x = {"equal": np.ones(c.blocks), "few": rng.integers(0, 5, c.blocks),
+         "steep": 2.0 ** -rng.integers(0, 100, c.blocks), "zeros": np.where(rng.random(c.blocks) < 0.9, 0, 1),
+         "outlier": np.where(np.arange(c.blocks) == 7, 1e30, rng.random(c.blocks)),
+         "tiny": rng.integers(0, 100, c.blocks) * 2.0**-133, "close": np.ones(c.blocks),
+         "huge": rng.integers(-200, 200, c.blocks) * 2.0**120}[kind]
+    v[:] = torch.from_numpy(x.astype(np.float32)).to(torch.bfloat16).cuda()[:, None, None]
+    if kind == "close":  # apart by 2^-20 of the sum: far below what its parts could be off by
+        v[:, :, 0] = torch.from_numpy(rng.integers(0, 128, c.blocks).astype(np.float32) * 2.0**-20).cuda()[:, None]
+    q = c.make((batch, 2, D))
+    q.fill_({"tiny": 2.0**-120, "huge": 2.0**100}.get(kind, 0.5))
+    for keep in (10, 150, 299):
+        run_select(c, q, keep, 1, 2)
+
+
+@pytest.mark.parametrize("batch,blocks", [(1, 400), (1, 2600), (64, 400)])
+@pytest.mark.parametrize("D", [64, 96, 128])
+def test_select_bf16_ranks_nan_and_infinities(batch, blocks, D):
+    c = Cache(23, [blocks * 16] * batch, hkv=1, D=D)
+    sort_summaries(c)
+    v = c.summary[:, :c.sum_n].view(c.blocks, 2, D)
+    for i, x in ((11, math.nan), (30, math.inf), (50, -math.inf)):
+        for b in range(batch):
+            v[int(c.tables[b, i]), :, 5] = x
+    q = c.make((batch, 1, D))
+    q[:, :, 5] = 1.0
+    got = run_select(c, q, 6, 1, 1).cpu().numpy()
+    assert (got[:, 0] == 11).any(1).all() and (got[:, 0] == 30).any(1).all()
+    q[:, :, 7] = math.inf  # finite rows decide by the sign of one channel
+    run_select(c, q, 6, 1, 1)
+    q[:, :, 9] = math.nan  # every score is NaN: the lowest blocks
+    got = run_select(c, q, 6, 1, 1).cpu().numpy()
+    assert (got == [0, 1, 2, 3, 4, blocks - 1]).all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("pad,offset,extra", [(8, 0, 0), (1, 0, 0), (0, 1, 0), (0, 0, 3), (0, 0, 64)])
 def test_select_over_strides_and_alignments(dtype, pad, offset, extra):
