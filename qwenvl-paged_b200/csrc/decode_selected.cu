@@ -11,7 +11,7 @@
 //
 // Measured (bf16, head_dim 128, blocks of 16): 128 listed blocks of 32 contexts
 // with 8 kv heads, 269 MB, 48.0 us, 5.6 TB/s; 64 of 64 ragged contexts with 4,
-// 134 MB, 27 us, 5.0 TB/s; 128 of one context, 8.6 us. fp32: 33 of 9 contexts
+// 134 MB, 27 us, 5.0 TB/s; 128 of one context, 8.1 us. fp32: 33 of 9 contexts
 // (4 MB) 7.8 us; 64 of 64 with head_dim 128, 268 MB, 76 us, where the issue
 // slots are the limit (54 % busy at 21 % of the warps).
 #include "attention_tile.cuh"
@@ -115,12 +115,16 @@ struct TileShape {
     static constexpr uint32_t kRing = kStages * kPiece;              // one warp's
     static constexpr uint32_t kBars = kTileWarps * kRing;            // offset of the barriers
     static constexpr uint32_t kStats = kBars + kTileWarps * kStages * 8;  // m, l of 16 rows per warp, tokens seen
+    static constexpr uint32_t kWeights = kStats + kTileWarps * (32 * 4 + 16);  // of every warp's sums, by row
+    static constexpr uint32_t kSums = kWeights + Tile::kHeads * kTileWarps * 4;  // of the CTA's weights, by row
     // of every CTA of a cluster: m and l of its rows, and its sums of the
     // columns that this CTA writes out
-    static constexpr uint32_t kRanks = kStats + kTileWarps * (32 * 4 + 16);
+    static constexpr uint32_t kRanks = kSums + Tile::kHeads * 4;
     static constexpr uint32_t kShare = kRanks + kMaxCluster * Tile::kHeads * 8;
-    static constexpr uint32_t kPairs = Tile::kHeads * Tile::kDim / 2;
-    static constexpr uint32_t kSmem = kShare + (kPairs + kMaxCluster * kMaxCluster) * 8 + 1024;
+    static constexpr uint32_t kPairs = Tile::kHeads * (Tile::kDim <= 64 ? 32 : 64);  // a power of two
+    static constexpr uint32_t kSmem = kShare + kPairs * 8 + 1024;
+    static_assert(kTileWarps == 4, "a row's weights are a float4");
+    static_assert(kTileThreads >= kMaxCluster * Tile::kHeads, "a thread per row of every CTA");
     static_assert(kRing >= Tile::kHeads * Tile::kDim * 4, "a warp's partial output takes the place of its ring");
     static_assert(kPiece % 1024 == 0 && kStages <= 8, "pieces start on swizzle boundaries, their counts fit 64 bits");
 };
@@ -455,67 +459,92 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         if (lane == 0) reinterpret_cast<uint32_t*>(stat)[32] = seen;
     }
     __syncthreads();
-    // Join the warps, two elements a thread: straight to the output, or to the
-    // CTA of the cluster that writes them out. A CTA that attended no token
-    // says so by a negative sum.
+    // Join the warps. A CTA that attended no token says so by a negative sum.
     const float* stats = reinterpret_cast<const float*>(smem + S::kStats);
-    T* out = static_cast<T*>(p.out) + (static_cast<size_t>(b) * p.hq + h0) * D;
-    uint32_t any = 0;
+    float4* weights = reinterpret_cast<float4*>(smem + S::kWeights);
+    float* own_sums = reinterpret_cast<float*>(smem + S::kSums);
+    if (cluster > 1) cg::this_cluster().barrier_wait();  // every CTA has started: its memory can be written
+    {
+        const uint32_t g = threadIdx.x % Tile::kHeads, r = threadIdx.x / Tile::kHeads;
+        uint32_t any = 0;
+        float M = -INFINITY, sum = 0.f, w[kTileWarps];
 #pragma unroll
-    for (int w = 0; w < kTileWarps; ++w) any |= reinterpret_cast<const uint32_t*>(stats)[w * 36 + 32];
+        for (int i = 0; i < kTileWarps; ++i) {
+            any |= reinterpret_cast<const uint32_t*>(stats)[i * 36 + 32];
+            M = fmaxf(M, stats[i * 36 + g]);
+        }
+#pragma unroll
+        for (int i = 0; i < kTileWarps; ++i) {
+            w[i] = partial_weight(stats[i * 36 + g], M);
+            sum += w[i] * stats[i * 36 + 16 + g];
+        }
+        if (any == 0) sum = -1.f;
+        if (r == 0) {
+            weights[g] = make_float4(w[0], w[1], w[2], w[3]);
+            own_sums[g] = sum;
+        }
+        if (cluster > 1 && r < cluster)
+            reinterpret_cast<float2*>(cg::this_cluster().map_shared_rank(smem, r) +
+                                      S::kRanks)[rank * Tile::kHeads + g] = make_float2(M, sum);
+    }
+    __syncthreads();
+    // Two elements a thread: straight to the output, or to the CTA of the
+    // cluster that writes them out.
+    T* out = static_cast<T*>(p.out) + (static_cast<size_t>(b) * p.hq + h0) * D;
     auto write_out = [&](uint32_t g, uint32_t d, float x, float y, float sum) {
         const float inv = 1.f / sum;
         *reinterpret_cast<uint32_t*>(out + g * D + d) = sum < 0.f ? 0u : pack_bf16x2(x * inv, y * inv);
     };
     const uint32_t pairs = static_cast<uint32_t>(G) * (D / 2);
-    const uint32_t share = (pairs + cluster - 1) / cluster;  // pairs that a CTA writes out
-    if (cluster > 1) cg::this_cluster().barrier_wait();      // every CTA has started: its memory can be written
+    uint32_t shift = 0;  // a CTA writes out 2^shift pairs
+    while (cluster << shift < pairs) ++shift;
+    const uint32_t share = 1u << shift;
+#pragma unroll 4
     for (uint32_t i = threadIdx.x; i < pairs; i += kTileThreads) {
         const uint32_t g = i / (D / 2), d = i % (D / 2) * 2;
-        float M = -INFINITY;
+        const float4 w = weights[g];
+        float2 o[kTileWarps];
 #pragma unroll
-        for (int w = 0; w < kTileWarps; ++w) M = fmaxf(M, stats[w * 36 + g]);
-        float sum = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-        for (int w = 0; w < kTileWarps; ++w) {
-            const float2 o = *reinterpret_cast<const float2*>(smem + w * S::kRing + (g * D + d) * 4);
-            const float weight = partial_weight(stats[w * 36 + g], M);
-            sum += weight * stats[w * 36 + 16 + g];
-            x += weight * o.x;
-            y += weight * o.y;
-        }
-        if (any == 0) sum = -1.f;
-        if (cluster == 1) {
-            write_out(g, d, x, y, sum);
-        } else {
-            uint8_t* to = cg::this_cluster().map_shared_rank(smem, i / share);
-            reinterpret_cast<float2*>(to + S::kShare)[rank * share + i % share] = make_float2(x, y);
-            if (d == 0)
-                for (uint32_t r = 0; r < cluster; ++r)
-                    reinterpret_cast<float2*>(cg::this_cluster().map_shared_rank(smem, r) +
-                                              S::kRanks)[rank * Tile::kHeads + g] = make_float2(M, sum);
-        }
+        for (int k = 0; k < kTileWarps; ++k)
+            o[k] = *reinterpret_cast<const float2*>(smem + k * S::kRing + (g * D + d) * 4);
+        const float x = fmaf(w.w, o[3].x, fmaf(w.z, o[2].x, fmaf(w.y, o[1].x, w.x * o[0].x)));
+        const float y = fmaf(w.w, o[3].y, fmaf(w.z, o[2].y, fmaf(w.y, o[1].y, w.x * o[0].y)));
+        if (cluster == 1)
+            write_out(g, d, x, y, own_sums[g]);
+        else
+            reinterpret_cast<float2*>(cg::this_cluster().map_shared_rank(smem, i >> shift) +
+                                      S::kShare)[rank * share + i % share] = make_float2(x, y);
     }
     if (cluster == 1) return;
     cg::this_cluster().sync();
+    const float2* rows = reinterpret_cast<const float2*>(smem + S::kRanks);
+    const float2* sums = reinterpret_cast<const float2*>(smem + S::kShare);
     for (uint32_t k = threadIdx.x; k < share; k += kTileThreads) {
         const uint32_t i = rank * share + k;
         if (i >= pairs) break;
         const uint32_t g = i / (D / 2), d = i % (D / 2) * 2;
-        const float2* rows = reinterpret_cast<const float2*>(smem + S::kRanks);
-        const float2* sums = reinterpret_cast<const float2*>(smem + S::kShare);
+        float2 row[kMaxCluster], o[kMaxCluster];
         float M = -INFINITY;
-        for (uint32_t r = 0; r < cluster; ++r) M = fmaxf(M, rows[r * Tile::kHeads + g].x);
+#pragma unroll
+        for (uint32_t r = 0; r < kMaxCluster; ++r) {
+            row[r] = make_float2(-INFINITY, -1.f);
+            o[r] = make_float2(0.f, 0.f);
+            if (r < cluster) {
+                row[r] = rows[r * Tile::kHeads + g];
+                o[r] = sums[r * share + k];
+            }
+            M = fmaxf(M, row[r].x);
+        }
         float sum = 0.f, x = 0.f, y = 0.f;
         bool none = true;
-        for (uint32_t r = 0; r < cluster; ++r) {
-            const float2 row = rows[r * Tile::kHeads + g], o = sums[r * share + k];
-            if (row.y < 0.f) continue;
-            const float weight = partial_weight(row.x, M);
-            none = false;
-            sum += weight * row.y;
-            x += weight * o.x;
-            y += weight * o.y;
+#pragma unroll
+        for (uint32_t r = 0; r < kMaxCluster; ++r) {
+            const bool empty = row[r].y < 0.f;
+            const float weight = empty ? 0.f : partial_weight(row[r].x, M);
+            none &= empty;
+            sum += empty ? 0.f : weight * row[r].y;
+            x += empty ? 0.f : weight * o[r].x;
+            y += empty ? 0.f : weight * o[r].y;
         }
         write_out(g, d, x, y, none ? -1.f : sum);
     }
@@ -1120,7 +1149,7 @@ extern "C" int qvp_decode_selected(const qvp_decode_selected_args* args, qvp_str
         p.cluster = 1;
         // Two CTAs are resident per SM: split a list while the whole grid still
         // is (256 lists of 128 blocks: 47 us whole, 52 us in two; 8 lists of
-        // 128 blocks: 25 us whole, 8.4 us in eight).
+        // 128 blocks: 25 us whole, 8.1 us in eight).
         while (p.cluster < kMaxCluster && segments * p.cluster * 2 <= 2 * sms && pieces > kTileWarps * p.cluster)
             p.cluster *= 2;
         return p.D == 128  ? launch_tile<128>(p, a, static_cast<uint32_t>(segments), st)
