@@ -492,6 +492,20 @@ def test_select_where_ctas_share_a_context(dtype, D, pad, blocks, batch):
         run_select(c, q, keep, sink, recent)
 
 
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("bf16", 80), ("f32", 64), ("f32", 33)])
+@pytest.mark.parametrize("blocks", [1500, 5000])
+def test_select_short_contexts_in_a_call_for_long_ones(dtype, D, blocks):
+    """max_context_len is a bound, as a captured graph has it: most CTAs of a context then have no block."""
+    keep = 7
+    ctx = [keep * 16 + 1, (keep + 2) * 16, 0, 16 * 16, 1, 300 * 16 + 5]
+    c = Cache(24, ctx, dtype=dtype, hkv=2, D=D, pitch=blocks)
+    sort_summaries(c)
+    q = c.make((len(ctx), 8, D))
+    run_select(c, q, keep, 1, 2, max_context_len=blocks * 16)
+    run_select(c, q, keep, 0, 0, max_context_len=blocks * 16)
+    run_select(c, q, 1, 0, 0, max_context_len=blocks * 16)
+
+
 @pytest.mark.parametrize("kind", ["equal", "few", "steep", "zeros", "outlier", "tiny", "close", "huge"])
 @pytest.mark.parametrize("batch,blocks", [(1, 1500), (1, 2600), (64, 300)])
 @pytest.mark.parametrize("D", [64, 128])
