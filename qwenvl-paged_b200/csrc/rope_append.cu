@@ -9,14 +9,14 @@
 //
 // Every q, k and v element is read once and written once: the call is bound
 // by HBM for prompts and by latency for single tokens. A CTA takes the new
-// tokens of one cache block (so a block's summary belongs to one CTA) and
-// either its K and V or some of its query heads. It makes the cosines and sines
+// tokens of one cache block (so the summary of a block's head belongs to one
+// CTA) and either K and V of some kv heads or some query heads. It makes the cosines and sines
 // of its tokens once for all heads, in shared memory; then each thread goes
 // through the heads with those of its run of pairs of one token in registers,
 // the next heads on their way in registers or in shared memory.
 //
 // Measured (28 + 4 + 4 heads of 128, bf16): 16 prompts of 2,048 tokens, 609 MB,
-// 110.9 us, 5.5 TB/s; 64 single tokens 5.3 us. 7 ragged fp32 chunks, 11 MB: 7.9
+// 110.9 us, 5.5 TB/s; 64 single tokens 5.7 us. 7 ragged fp32 chunks, 11 MB: 7.9
 // us. 16 tokens at a time instead of 8 took 120 us for the prompts through
 // registers, 4 took 123.
 #include "sparse_common.cuh"
@@ -53,7 +53,9 @@ struct RopeParams {
     uint32_t hq, hkv, D;
     uint32_t batch, max_q;
     uint32_t units;          // cache blocks a sequence's new tokens can touch
-    uint32_t heads_per_cta;  // query heads of a CTA with blockIdx.y > 0
+    uint32_t heads_per_cta;  // query heads of a CTA
+    uint32_t kv_per_cta;     // or kv heads
+    uint32_t kv_groups;
     uint32_t tokens;         // tokens of a CTA at a time
     uint32_t rotary;
     bool interleaved;
@@ -218,12 +220,14 @@ struct HeadRing {
 };
 
 // VEC elements at a time where rows and halves fall on 16-byte boundaries,
-// else one by one. grid (batch * units, 1 + groups of query heads). RING: heads
-// on their way in shared memory, and keys and values last, so that the long
-// CTAs do not start last; else in registers, and keys and values first, whose
-// way through table and summary is the longest.
+// else one by one. grid (batch * units, groups of kv heads + groups of query
+// heads). RING: heads on their way in shared memory, and one group of kv heads,
+// the shortest CTAs, last; else in registers, and kv heads first, whose way
+// through table and summary is the longest. Seven CTAs fit an SM with up to 72
+// registers a thread: the compiler takes 70 for the ring by itself, and up to 87
+// for the other, which cost 2 prompts of 2,048 tokens 26.1 us instead of 23.4.
 template <typename T, int VEC, bool RING>
-__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads, RING ? 0 : 7) rope_append_kernel(const RopeParams p) {
     // of pair it * VEC + j of token t at [j][t * row_items + it], rows one apart
     // from a multiple of the banks
     __shared__ float2 table[kRopeTokens * kMaxPairs + VEC];
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
     const uint32_t lo = max(first, base);                                       // new positions [lo, hi)
     const uint32_t hi = min(static_cast<uint32_t>(ctx), base + p.T);
 
-    const bool kv = blockIdx.y == (RING ? gridDim.y - 1 : 0);
+    const bool kv = RING ? blockIdx.y == gridDim.y - 1 : blockIdx.y < p.kv_groups;
     uint8_t* frame = nullptr;
     int32_t id = 0;
     if (kv) {
@@ -268,15 +272,19 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
     const size_t row0 = static_cast<size_t>(b) * p.max_q + (lo - first);        // token row of position lo
     const uint32_t cnt = hi - lo;
     const uint32_t half = p.rotary / 2;
-    const uint32_t h0 = kv ? 0 : (RING ? blockIdx.y : blockIdx.y - 1) * p.heads_per_cta;
-    const uint32_t nh = kv ? p.hkv : min(p.heads_per_cta, p.hq - h0);
-    const T* src = kv ? static_cast<const T*>(p.k) + row0 * p.k_pitch
-                      : static_cast<const T*>(p.q) + row0 * p.q_pitch + static_cast<size_t>(h0) * D;
+    // heads [h0, h0 + nh)
+    const uint32_t h0 = kv ? (RING ? 0 : blockIdx.y * p.kv_per_cta)
+                           : (RING ? blockIdx.y : blockIdx.y - p.kv_groups) * p.heads_per_cta;
+    const uint32_t nh = !kv ? min(p.heads_per_cta, p.hq - h0) : RING ? p.hkv : min(p.kv_per_cta, p.hkv - h0);
+    const size_t col = static_cast<size_t>(h0) * D;                             // of the first head in a token
+    const size_t kv_col = RING ? 0 : col;
+    const T* src = kv ? static_cast<const T*>(p.k) + row0 * p.k_pitch + kv_col
+                      : static_cast<const T*>(p.q) + row0 * p.q_pitch + col;
     const size_t src_pitch = kv ? p.k_pitch : p.q_pitch;
-    T* dst = kv ? kslots + (lo - base) * slot_elems
+    T* dst = kv ? kslots + (lo - base) * slot_elems + kv_col
                 : static_cast<T*>(p.q_out) + (row0 * p.hq + h0) * static_cast<size_t>(D);
     const size_t dst_pitch = kv ? slot_elems : static_cast<size_t>(p.hq) * D;
-    const T* v = static_cast<const T*>(p.v) + row0 * p.v_pitch;
+    const T* v = static_cast<const T*>(p.v) + row0 * p.v_pitch + kv_col;
     // a thread's place: an item of a token, and the heads it shares with the
     // threads at the same place
     const uint32_t places = p.tokens * row_items;
@@ -330,11 +338,11 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
         }
     }
     if (kv) {
-        const uint32_t v_items = static_cast<uint32_t>(slot_elems / VEC);
+        const uint32_t v_items = RING ? static_cast<uint32_t>(slot_elems / VEC) : nh * D / VEC;
 #pragma unroll 4
         for (uint32_t i = threadIdx.x; i < cnt * v_items; i += kRopeThreads) {
             const uint32_t t = i / v_items, e = (i % v_items) * VEC;
-            store_vec<T, VEC>(vslots + (lo - base + t) * slot_elems + e, load_vec<T, VEC>(v + t * p.v_pitch + e));
+            store_vec<T, VEC>(vslots + (lo - base + t) * slot_elems + kv_col + e, load_vec<T, VEC>(v + t * p.v_pitch + e));
         }
     }
     if (!kv || p.summary == nullptr) return;
@@ -344,7 +352,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
     __syncthreads();
     const uint32_t filled = min(p.T, static_cast<uint32_t>(ctx) - base);
     // a thread owns one item of one kv head and every groups-th slot
-    const uint32_t k_items = p.hkv * row_items;
+    const uint32_t k_items = (RING ? p.hkv : nh) * row_items;
     uint32_t groups = 1;
     while (groups < kRopeTokens && groups * 2 * k_items <= kRopeThreads) groups *= 2;
     T* bounds = reinterpret_cast<T*>(p.summary + static_cast<size_t>(id) * p.summary_stride) +
@@ -360,7 +368,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
         start_range(lo1, hi1);
         if (live) {
             for (uint32_t s = g; s < filled; s += groups) {
-                const T* src = kslots + s * slot_elems + static_cast<size_t>(h) * D;
+                const T* src = kslots + s * slot_elems + kv_col + static_cast<size_t>(h) * D;
                 const Vec<T, VEC> u = load_vec<T, VEC>(src + x.e0);
                 widen(lo0, hi0, u, u);
                 if (two) {
@@ -383,7 +391,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopePar
             }
         }
         if (live && g == 0) {
-            T* dst = bounds + static_cast<size_t>(h) * 2 * D;
+            T* dst = bounds + 2 * kv_col + static_cast<size_t>(h) * 2 * D;
             store_vec<T, VEC>(dst + x.e0, lo0);
             store_vec<T, VEC>(dst + D + x.e0, hi0);
             if (two) {
@@ -512,8 +520,6 @@ extern "C" int qvp_rope_append(const qvp_rope_append_args* args, qvp_stream_t st
     while (groups * 4 < a.num_query_heads && static_cast<uint64_t>(p.units) * a.batch * groups < 4 * sms) groups *= 2;
     p.heads_per_cta = groups > 0 ? ceil_div(a.num_query_heads, groups) : 0;
     if (groups > 0) groups = ceil_div(a.num_query_heads, p.heads_per_cta);
-    const dim3 grid(p.units * a.batch, 1 + groups);
-
     const uint32_t V = 16 / elem;
     const bool vec = D % (2 * V) == 0 && a.rotary_dim % (2 * V) == 0 && aligned_to(a.pool, 16) &&
                      a.block_stride % 16 == 0 && aligned_to(a.key, 16) && aligned_to(a.value, 16) &&
@@ -522,14 +528,25 @@ extern "C" int qvp_rope_append(const qvp_rope_append_args* args, qvp_stream_t st
                       (aligned_to(a.query, 16) && aligned_to(a.query_out, 16) && q_pitch % V == 0)) &&
                      (a.summary == nullptr || (aligned_to(a.summary, 16) && a.summary_stride % 16 == 0));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    // Heads through shared memory where a thread has at least a ring of them and
-    // CTAs come in waves: 16 prompts of 2,048 tokens (28 + 4 + 4 heads of 128,
-    // bf16) 110.9 us, 116.2 through registers; 32 of 512: 59.3 and 65.9. Else
-    // registers: 2 prompts of 2,048 23.0 us, 26.8 through shared memory; 1,024
-    // single tokens 12.0 and 13.2.
+    // Heads through shared memory where a thread has at least a ring of them,
+    // query heads are most of the work and CTAs come in waves: 16 prompts of 2,048
+    // tokens (28 + 4 + 4 heads of 128, bf16) 110.9 us, 116.2 through registers; 32
+    // of 512: 59.3 and 65.9. Else registers: 2 prompts of 2,048 23.0 us, 26.8
+    // through shared memory; 1,024 single tokens 12.0 and 13.2; 13 fp32 prompts
+    // with 8 + 8 + 8 heads 59.1 and 73.3.
     const uint32_t places = p.tokens * (D / (2 * V));
     const uint32_t sharers = places > 0 && places < kRopeThreads ? kRopeThreads / places : 1;
-    const bool ring = p.heads_per_cta >= kRing * sharers && static_cast<uint64_t>(grid.x) * grid.y > 8 * sms;
+    const bool ring = p.heads_per_cta >= kRing * sharers && p.heads_per_cta > 3 * sh.num_kv_heads &&
+                      static_cast<uint64_t>(p.units) * a.batch * (1 + groups) > 8 * sms;
+    // The kv heads of a block are split while the grid would leave SMs without
+    // work (every head has its part of the summary): 3 chunks of 13 tokens with 8
+    // kv heads 6.4 us, 11.4 with all in a CTA.
+    uint32_t kv_groups = 1;
+    while (!ring && kv_groups < sh.num_kv_heads && static_cast<uint64_t>(p.units) * a.batch * kv_groups * 2 <= sms)
+        kv_groups *= 2;
+    p.kv_per_cta = ceil_div(sh.num_kv_heads, kv_groups);
+    p.kv_groups = ceil_div(sh.num_kv_heads, p.kv_per_cta);
+    const dim3 grid(p.units * a.batch, p.kv_groups + groups);
     return a.dtype == QVP_DTYPE_F32 ? launch_rope<float>(p, vec, ring, grid, st)
                                     : launch_rope<__nv_bfloat16>(p, vec, ring, grid, st);
 }
