@@ -464,9 +464,10 @@ extern "C" int qvp_rope_append(const qvp_rope_append_args* args, qvp_stream_t st
         if (!aligned_to(a.query, elem) || !aligned_to(a.query_out, elem))
             return fail(QVP_ERR_INVALID, "query or query_out is not element-aligned");
     }
-    qvp_block_shape ss;
-    qvp_summary_shape(&sh, &ss);
     if (a.summary != nullptr) {
+        qvp_block_shape ss;
+        rc = qvp_summary_shape(&sh, &ss);
+        if (rc != QVP_OK) return rc;
         rc = check_pool("summary pool", a.summary, a.summary_stride, qvp_block_bytes(&ss), elem, a.num_blocks);
         if (rc != QVP_OK) return rc;
     }

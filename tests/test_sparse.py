@@ -135,6 +135,18 @@ def test_blocks_past_32_bits_of_elements_are_refused(call, pool):
     assert "elements" in qvp.last_error()
 
 
+@pytest.mark.parametrize("call", [_append, _summarize, _select])
+def test_summaries_past_32_bits_of_rows_are_refused(call):
+    # 2^31 layers of 2 kv heads; the layers alone still fit the shape
+    deep = qvp.make_shape(1, 2**31, 2, 8, 2)
+    where = {} if call is _select else dict(block_stride=qvp.block_stride(deep))
+    if call is _append:
+        where.update(rotary_dim=8, rope_sections=[1, 1, 2])
+    for stride in (8, 256, 2**37, 2**63):  # none is a summary block's size
+        assert call(shape=deep, layer=0, num_blocks=1, summary_stride=stride, **where) == qvp.ERR_UNSUPPORTED
+        assert "layer" in qvp.last_error()
+
+
 def test_select_refuses_contexts_that_do_not_fit_a_cluster():
     blocks = 8 * 20480 + 2
     assert _select(max_blocks_per_seq=blocks + 1, max_context_len=(blocks + 1) * 16) == qvp.ERR_UNSUPPORTED
