@@ -346,8 +346,9 @@ QVP_API int qvp_kv_append(void* pool, size_t block_stride, uint32_t num_blocks,
  * past the context; 4: a length out of range) and are skipped, so no access
  * leaves the pool. QVP_ERR_UNSUPPORTED answers shapes past the kernels'
  * counters: head_dim above 256, a batch above 65535, blocks of more than 65536
- * tokens or 2^31 - 1 elements of K in a layer. The block id -1 past a context is never read. No
- * counterpart in the reference (it attends every token).
+ * tokens or 2^31 - 1 elements of K in a layer, more than 2^32 - 1 (layer, kv
+ * head) pairs, pools whose size passes 64 bits. The block id -1 past a context
+ * is never read. No counterpart in the reference (it attends every token).
  * ------------------------------------------------------------------------- */
 
 /* The block shape of the summary pool of a cache with blocks of `shape`. */

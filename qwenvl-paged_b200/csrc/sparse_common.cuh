@@ -127,6 +127,10 @@ inline int check_shape(const qvp_block_shape& sh, int32_t dtype, uint32_t layer)
     // elements within a block's K are counted in 32 bits
     if (static_cast<uint64_t>(sh.tokens_per_block) * sh.num_kv_heads * sh.head_dim > 0x7fffffffu)
         return fail(QVP_ERR_UNSUPPORTED, "blocks of more than 2^31 - 1 elements of K in a layer");
+    // the rows of a summary pool are counted in 32 bits; a block then has below
+    // 2^59 bytes (2^16 tokens, 2^32 rows, 2^8 elements), so its size does not wrap
+    if (static_cast<uint64_t>(sh.num_layers) * sh.num_kv_heads > 0xffffffffu)
+        return fail(QVP_ERR_UNSUPPORTED, "more than 2^32 - 1 (layer, kv head) pairs");
     return QVP_OK;
 }
 
@@ -138,6 +142,7 @@ inline int check_pool(const char* name, const void* base, size_t stride, size_t 
     if (!aligned_to(base, elem) || stride % elem != 0) return fail(QVP_ERR_INVALID, "%s is not element-aligned", name);
     if (num_blocks == 0) return fail(QVP_ERR_INVALID, "empty %s", name);
     if (num_blocks > 0x7fffffffu) return fail(QVP_ERR_UNSUPPORTED, "%s of more than 2^31 blocks", name);
+    if (stride > SIZE_MAX / num_blocks) return fail(QVP_ERR_UNSUPPORTED, "%s of more than 2^64 bytes", name);
     return QVP_OK;
 }
 

@@ -147,6 +147,24 @@ def test_summaries_past_32_bits_of_rows_are_refused(call):
         assert "layer" in qvp.last_error()
 
 
+@pytest.mark.parametrize("call", [_append, _attend])
+def test_blocks_whose_size_wraps_are_refused(call):
+    # 2^16 tokens x 2^31 layers x 2^6 heads x 2^8 elements x K and V x 4 bytes = 2^64: any stride would do
+    wraps = qvp.make_shape(65536, 2**31, 64, 256, 4)
+    assert qvp.block_bytes(wraps) == 0
+    where = dict(summary=0, rotary_dim=0, max_query_len=1) if call is _append else {}
+    assert call(shape=wraps, layer=2**30, dtype=qvp.DTYPE_F32, num_query_heads=64, block_stride=256,
+                **where) == qvp.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("call,stride", [(_append, "block_stride"), (_append, "summary_stride"),
+                                         (_summarize, "block_stride"), (_summarize, "summary_stride"),
+                                         (_select, "summary_stride"), (_attend, "block_stride")])
+def test_pools_whose_size_wraps_are_refused(call, stride):
+    assert call(num_blocks=2**30, **{stride: 2**34}) == qvp.ERR_UNSUPPORTED
+    assert "bytes" in qvp.last_error()
+
+
 def test_select_refuses_contexts_that_do_not_fit_a_cluster():
     blocks = 8 * 20480 + 2
     assert _select(max_blocks_per_seq=blocks + 1, max_context_len=(blocks + 1) * 16) == qvp.ERR_UNSUPPORTED
