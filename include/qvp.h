@@ -385,7 +385,10 @@ QVP_API int qvp_summary_shape(const qvp_block_shape* shape, qvp_block_shape* sum
  * >= query_lens[b] are neither read nor written, and query_lens[b] = 0 leaves
  * a sequence out. num_query_heads = 0 appends keys and values only;
  * rotary_dim = 0 rotates nothing. The blocks written must belong to one
- * sequence of the call each (copy-on-write first).
+ * sequence of the call each (copy-on-write first). A length out of range
+ * leaves out its sequence, query_out included; an id outside the pool leaves
+ * out the keys, values and summary of its block, while query_out, which needs
+ * no block, is written.
  */
 #define QVP_ROPE_MAX_AXES 4
 typedef struct qvp_rope_append_args {

@@ -342,6 +342,47 @@ def test_append_flags_bad_lengths_and_ids_and_serves_the_rest(change, bit):
     assert np.array_equal(after[block].reshape(2, 16, 64)[:, :4], want)
 
 
+@pytest.mark.parametrize("change,bit", [
+    (dict(ctx=[-1, 20]), 4), (dict(ctx=[65, 20]), 4), (dict(ctx=[9, 20]), 4), (dict(new=[-1, 4]), 4),
+    (dict(new=[13, 4]), 4), (dict(table=-1), 1), (dict(table=10**6), 1)])
+@pytest.mark.parametrize("dtype,hq,hkv", [("bf16", 6, 3), ("f32", 4, 1)])
+def test_append_leaves_queries_and_summaries_of_bad_lengths_alone(change, bit, dtype, hq, hkv):
+    """A bad length leaves out its sequence; a bad id leaves out its block, whose queries are rotated all the same."""
+    torch = _torch()
+    c = Cache(40, [40, 20], dtype=dtype, hkv=hkv, D=64, pitch=4)
+    q, k, v = (c.make((2, 12, h, 64)) for h in (hq, hkv, hkv))
+    freq = torch.from_numpy((1e4 ** (-np.arange(32) / 32)).astype(np.float32)).cuda()
+    before = [c.pool.clone(), c.summary.clone(), c.make((2, 12, hq, 64))]
+
+    def append(ctx, new, pool, summary, out):
+        ctx, new = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (ctx, new))
+        c.pool, c.summary = pool, summary
+        args = qvp.rope_append_args(**c.common(context_lens=ctx.data_ptr()), **c.at_pool(), **c.at_summary(),
+                                    num_query_heads=hq, max_query_len=12, query_lens=new.data_ptr(),
+                                    query=q.data_ptr(), key=k.data_ptr(), value=v.data_ptr(),
+                                    query_out=out.data_ptr(), rotary_dim=64, inv_freq=freq.data_ptr())
+        assert qvp.rope_append(args, _stream()) == qvp.OK
+        return c.errors()
+
+    good = [x.clone() for x in before]
+    assert append([40, 20], [10, 4], *good) == 0
+    if "table" in change:
+        c.tables_d[0, 2] = change["table"]
+    got = [x.clone() for x in before]
+    assert append(change.get("ctx", [40, 20]), change.get("new", [10, 4]), *got) == bit
+    served = [int(c.tables[1, 1])]               # tokens 16 .. 19 of the second sequence
+    if bit == 1:
+        served.append(int(c.tables[0, 1]))       # tokens 30 and 31 of the first: 32 .. 39 have no block
+    for i in range(2):
+        want = before[i].clone()
+        want[served] = good[i][served]
+        assert np.array_equal(_bits(got[i]), _bits(want))
+    want = good[2].clone()
+    if bit == 4:
+        want[0] = before[2][0]
+    assert np.array_equal(_bits(got[2]), _bits(want))
+
+
 # --- summaries -----------------------------------------------------------------
 
 
