@@ -170,6 +170,17 @@ def test_select_refuses_contexts_that_do_not_fit_a_cluster():
     assert _select(max_blocks_per_seq=blocks + 1, max_context_len=(blocks + 1) * 16) == qvp.ERR_UNSUPPORTED
 
 
+@pytest.mark.parametrize("sink,recent", [(1, 1), (0, 0), (0, 3)])
+def test_select_refuses_one_block_past_its_longest_context(sink, recent):
+    # 114,688 blocks between sink and recent are served; the GPU tests launch that many
+    blocks = 114688 + sink + recent + 1
+    for tokens in (16, 1):
+        shape = qvp.make_shape(tokens, 2, 2, 64, 2)
+        assert _select(shape=shape, sink_blocks=sink, recent_blocks=recent, max_blocks_per_seq=blocks,
+                       max_context_len=(blocks - 1) * tokens + 1) == qvp.ERR_UNSUPPORTED
+        assert "114688" in qvp.last_error()
+
+
 @pytest.mark.parametrize("call", [_select, _attend])
 @pytest.mark.parametrize("entries", [2**31, 2**32 - 1])
 def test_lists_past_31_bits_are_refused(call, entries):

@@ -479,6 +479,16 @@ def test_select_over_long_contexts(blocks, keep, batch):
     run_select(c, c.make((batch, 4, c.D)), keep, 1, 0)
 
 
+@pytest.mark.parametrize("dtype,D", [("bf16", 64), ("f32", 16)])
+@pytest.mark.parametrize("blocks,ctx", [(114688, [114690, 100, 101, 102, 5000, 0]),      # eight CTAs, each full
+                                        (14336, [14338] + [90] * 80 + [130, 0] * 40),   # one CTA a context, full
+                                        (14337, [14339] + [90] * 80 + [130, 0] * 40)])  # a second one for the last block
+def test_select_where_ctas_hold_all_the_blocks_they_can(dtype, D, blocks, ctx):
+    c = Cache(39, ctx, dtype=dtype, hkv=1, D=D, T=1)
+    sort_summaries(c)
+    run_select(c, c.make((len(ctx), 3, D)), 100, 1, 1, max_context_len=blocks + 2)
+
+
 @pytest.mark.parametrize("kind", ["equal", "two", "few", "steep", "zeros", "outlier", "tiny"])
 @pytest.mark.parametrize("batch", [1, 64])
 def test_select_where_scores_tie_or_crowd(kind, batch):
