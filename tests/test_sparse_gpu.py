@@ -255,6 +255,16 @@ def test_append_long_chunks(new):
     run_append(c, new, 4, most=701)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("hkv,D", [(8, 128), (5, 64), (7, 80), (40, 64), (3, 33)])
+@pytest.mark.parametrize("kw", [dict(), dict(summary=False, fused=True), dict(hq=0)])
+def test_append_where_ctas_share_a_blocks_kv_heads(dtype, hkv, D, kw):
+    """Few blocks and many kv heads: even and uneven shares, old tokens of a block, an empty chunk."""
+    c = Cache(41, [13, 29, 0, 40], dtype=dtype, layers=2, layer=1, hkv=hkv, D=D)
+    kw = dict(kw)
+    run_append(c, [13, 9, 0, 1], kw.pop("hq", hkv), rotary=D // 4 * 2, **kw)
+
+
 @pytest.mark.parametrize("dtype,hq,hkv,D,T,most", [("bf16", 16, 4, 64, 8, 200), ("bf16", 17, 1, 64, 16, 400),
                                                    ("f32", 8, 2, 64, 16, 400), ("bf16", 12, 2, 256, 8, 200),
                                                    ("f32", 4, 1, 256, 8, 200), ("bf16", 10, 5, 96, 16, 400)])
