@@ -465,7 +465,9 @@ QVP_API int qvp_summarize_blocks(const qvp_summarize_args* args, qvp_stream_t st
  * all and reads no summary. The rest of the row is -1, and all of it for
  * context_lens[b] = 0. Scores are 64-bit sums, so the choice does not depend
  * on how the work is split. A score that is NaN (summaries or queries that
- * hold NaN, or infinities against zeros) counts as +infinity. The summaries
+ * hold NaN, or infinities against zeros) counts as +infinity. A block whose id
+ * is outside the pool sets error bit 1 and scores lowest; a context_lens entry
+ * out of range sets bit 4 and its lists are -1. The summaries
  * of blocks inside sink and recent are not read. Attention with a negative
  * scale would need the opposite score. max_context_len may span 114,688 blocks
  * between sink and recent; more are refused with QVP_ERR_UNSUPPORTED.
@@ -501,8 +503,9 @@ QVP_API int qvp_select_blocks(const qvp_select_args* args, qvp_stream_t stream);
  * twice counts twice; the order only changes the last bits. A list that
  * leaves no token (every entry < 0, or context_lens[b] = 0) gives zeros.
  * Entries past the context set error bit 1 and are skipped; a context_lens
- * entry out of range sets bit 4 and leaves out[b] as it was. Outputs are
- * the same bits from call to call. QVP_ERR_UNSUPPORTED answers lists of more
+ * entry out of range sets bit 4 and leaves out[b] as it was. Bit 2 says that
+ * a wait for a copy ran out (about a second): out is then not to be used.
+ * Outputs are the same bits from call to call. QVP_ERR_UNSUPPORTED answers lists of more
  * than 2^31 - 1 tokens and more than 2^28 (sequence, kv head) pairs. The dense
  * cache layout with head_dim 64, 96 or 128, bf16 and blocks of 8 or a multiple
  * of 16 tokens, query and out 4-byte aligned, runs on the tensor cores; every
