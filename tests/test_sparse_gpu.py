@@ -15,8 +15,11 @@ of it: 2^-8 of the value in bf16, 2^-24 in fp32 (STEP). To that comes:
   terms, they lose 2^-16; as one bf16, 2^-8.
 """
 import ctypes as C
+import importlib.util
 import itertools
 import math
+import os
+import random
 
 import numpy as np
 import pytest
@@ -1007,6 +1010,26 @@ def test_summaries_move_with_the_block_movers():
     c.tables[0], c.tables_d[0] = free, torch.from_numpy(free).cuda()
     c.summarize()
     assert c.errors() == 0 and torch.equal(moved, c.summary)
+
+
+@pytest.mark.parametrize("op", ["append", "summarize", "select", "attend"])
+def test_the_measured_cases_flag_nothing(op):
+    """The calls of perf/operators.py, its listed cases and drawn ones, leave their error words at zero."""
+    torch = _torch()
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "perf", "operators.py")
+    spec = importlib.util.spec_from_file_location("measured_operators", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    m.own = True
+    rng = random.Random(42)
+    cases = m.listed() + [m.draw(rng) for _ in range(24)]
+    for i, case in enumerate(c for c in cases if c["op"] == op):
+        state = m.prepare(case, i)
+        m.run(state)
+        torch.cuda.synchronize()
+        assert int(state["error"].item()) == 0, case
+        del state
+    torch.cuda.empty_cache()
 
 
 def test_offsets_past_32_bits():
