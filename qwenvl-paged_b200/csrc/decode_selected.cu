@@ -12,8 +12,11 @@
 // Measured (bf16, head_dim 128, blocks of 16): 128 listed blocks of 32 contexts
 // with 8 kv heads, 269 MB, 48.0 us, 5.6 TB/s; 64 of 64 ragged contexts with 4,
 // 134 MB, 27 us, 5.0 TB/s; 128 of one context, 8.1 us. fp32: 33 of 9 contexts
-// (4 MB) 7.8 us; 64 of 64 with head_dim 128, 268 MB, 76 us, where the issue
-// slots are the limit (54 % busy at 21 % of the warps).
+// (4 MB) 7.8 us; 64 of 64 with head_dim 128, 268 MB, 76 us (floor 41): 128
+// registers a thread leave four warps a scheduler, 1.2 of them ready, which wait
+// for fixed latencies, shared memory and the multiply-add pipe, hardly for HBM
+// (0.3 of 5.3 cycles an instruction), and 256 CTAs leave 40 of 148 SMs with one
+// CTA in place of two.
 #include "attention_tile.cuh"
 #include "sparse_common.cuh"
 

@@ -17,8 +17,11 @@
 //
 // Measured (28 + 4 + 4 heads of 128, bf16): 16 prompts of 2,048 tokens, 609 MB,
 // 110.9 us, 5.5 TB/s; 64 single tokens 5.7 us. 7 ragged fp32 chunks, 11 MB: 7.9
-// us. 16 tokens at a time instead of 8 took 120 us for the prompts through
-// registers, 4 took 123.
+// us. Furthest from their floors are grids of about one wave, where the time is
+// one CTA's chain (positions, angles, barrier, heads, V, summary): 1 prompt of
+// 2,048 tokens 17.5 us (floor 5.8), 2 23.4 (11.6), 8 of 512 23.3 (11.6), 1,024
+// single tokens 12.0 (3.2). 16 tokens at a time instead of 8 took 120 us for
+// the prompts through registers, 4 took 123.
 #include "sparse_common.cuh"
 
 namespace qvp {
@@ -225,7 +228,8 @@ struct HeadRing {
 // the shortest CTAs, last; else in registers, and kv heads first, whose way
 // through table and summary is the longest. Seven CTAs fit an SM with up to 72
 // registers a thread: the compiler takes 70 for the ring by itself, and up to 87
-// for the other, which cost 2 prompts of 2,048 tokens 26.1 us instead of 23.4.
+// for the other, which cost 2 prompts of 2,048 tokens 26.1 us instead of 23.4;
+// held to 72 it spills 8 bytes a thread in bf16 (none in fp32), gain included.
 template <typename T, int VEC, bool RING>
 __global__ void __launch_bounds__(kRopeThreads, RING ? 0 : 7) rope_append_kernel(const RopeParams p) {
     // of pair it * VEC + j of token t at [j][t * row_items + it], rows one apart
@@ -534,7 +538,12 @@ extern "C" int qvp_rope_append(const qvp_rope_append_args* args, qvp_stream_t st
     // tokens (28 + 4 + 4 heads of 128, bf16) 110.9 us, 116.2 through registers; 32
     // of 512: 59.3 and 65.9. Else registers: 2 prompts of 2,048 23.0 us, 26.8
     // through shared memory; 1,024 single tokens 12.0 and 13.2; 13 fp32 prompts
-    // with 8 + 8 + 8 heads 59.1 and 73.3.
+    // with 8 + 8 + 8 heads 59.1 and 73.3. Between those, 16 prompts of 2,048 take
+    // through shared memory and through registers: 16 + 4 + 4 heads 78.9 and 84.8
+    // in bf16, 148.0 and 149.8 in fp32; 24 + 8 + 8 127.4 and 135.0, 250.7 and
+    // 251.8; 16 + 8 + 8 105.5 and 115.4, 208.6 and 210.2 (32 fp32 prompts of 512:
+    // 115.0 and 112.4). The border of more than three query heads a kv head lies
+    // above the one that bf16 alone would have.
     const uint32_t places = p.tokens * (D / (2 * V));
     const uint32_t sharers = places > 0 && places < kRopeThreads ? kRopeThreads / places : 1;
     const bool ring = p.heads_per_cta >= kRing * sharers && p.heads_per_cta > 3 * sh.num_kv_heads &&
