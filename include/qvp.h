@@ -339,7 +339,8 @@ QVP_API int qvp_kv_append(void* pool, size_t block_stride, uint32_t num_blocks,
  *
  * None of the calls needs a workspace or keeps state, so calls on different
  * streams, and graphs that captured them, are independent as long as their
- * buffers are. All take the current device's pointers. dtype is the type of
+ * buffers are. All take the current device's pointers, each aligned to its
+ * element (QVP_ERR_INVALID otherwise). dtype is the type of
  * the pool, the summaries, q, k, v and the outputs; head_dim <= 256.
  * Lengths, tables and lists are read on the device only: entries that are
  * wrong set bits of *error_word (1: an id outside the pool or a list entry

@@ -984,6 +984,8 @@ extern "C" int qvp_select_blocks(const qvp_select_args* args, qvp_stream_t strea
     if (rc != QVP_OK) return rc;
     rc = check_tables(a.block_tables, a.context_lens, a.max_blocks_per_seq, a.batch);
     if (rc != QVP_OK) return rc;
+    rc = check_words(a.block_tables, a.context_lens, a.selected, a.error_word);
+    if (rc != QVP_OK) return rc;
     if (a.query == nullptr || a.selected == nullptr) return fail(QVP_ERR_INVALID, "null query or list pointer");
     if (!aligned_to(a.query, elem)) return fail(QVP_ERR_INVALID, "query is not element-aligned");
     const size_t q_row = static_cast<size_t>(a.num_query_heads) * sh.head_dim;

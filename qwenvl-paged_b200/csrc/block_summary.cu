@@ -122,6 +122,8 @@ extern "C" int qvp_summarize_blocks(const qvp_summarize_args* args, qvp_stream_t
     if (rc != QVP_OK) return rc;
     rc = check_tables(a.block_tables, a.context_lens, a.max_blocks_per_seq, a.batch);
     if (rc != QVP_OK) return rc;
+    rc = check_words(a.block_tables, a.context_lens, a.first_tokens, a.error_word);
+    if (rc != QVP_OK) return rc;
     if (a.max_context_len == 0) return fail(QVP_ERR_INVALID, "max_context_len is zero");
     if (a.max_context_len > token_capacity(a.max_blocks_per_seq, sh.tokens_per_block))
         return fail(QVP_ERR_INVALID, "max_context_len exceeds the table capacity");

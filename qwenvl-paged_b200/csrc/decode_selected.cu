@@ -1106,6 +1106,8 @@ extern "C" int qvp_decode_selected(const qvp_decode_selected_args* args, qvp_str
     if (rc != QVP_OK) return rc;
     rc = check_tables(a.block_tables, a.context_lens, a.max_blocks_per_seq, a.batch);
     if (rc != QVP_OK) return rc;
+    rc = check_words(a.block_tables, a.context_lens, a.selected, a.error_word);
+    if (rc != QVP_OK) return rc;
     if (a.query == nullptr || a.selected == nullptr || a.out == nullptr)
         return fail(QVP_ERR_INVALID, "null query, list or output pointer");
     if (!aligned_to(a.query, elem) || !aligned_to(a.out, elem))

@@ -448,6 +448,8 @@ extern "C" int qvp_rope_append(const qvp_rope_append_args* args, qvp_stream_t st
     if (rc != QVP_OK) return rc;
     rc = check_tables(a.block_tables, a.context_lens, a.max_blocks_per_seq, a.batch);
     if (rc != QVP_OK) return rc;
+    rc = check_words(a.block_tables, a.context_lens, a.query_lens, a.inv_freq, a.rope_positions, a.error_word);
+    if (rc != QVP_OK) return rc;
     if (a.query_lens == nullptr || a.key == nullptr || a.value == nullptr)
         return fail(QVP_ERR_INVALID, "null length, key or value pointer");
     if (a.max_query_len == 0 || a.max_query_len > 0x7fffffffu)

@@ -146,6 +146,14 @@ inline int check_pool(const char* name, const void* base, size_t stride, size_t 
     return QVP_OK;
 }
 
+// Arrays of 32-bit values that a kernel reads or writes one by one; null ones
+// are fine here.
+template <typename... P>
+int check_words(const P*... arrays) {
+    if ((... && aligned_to(arrays, 4))) return QVP_OK;
+    return fail(QVP_ERR_INVALID, "an int32 or float array is not 4-byte aligned");
+}
+
 inline int check_tables(const int32_t* tables, const int32_t* lens, uint32_t pitch, uint32_t batch) {
     if (tables == nullptr || lens == nullptr) return fail(QVP_ERR_INVALID, "null table or length pointer");
     if (pitch == 0) return fail(QVP_ERR_INVALID, "empty block table");

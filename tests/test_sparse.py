@@ -115,6 +115,16 @@ def test_decode_selected_refuses_inconsistent_arguments(bad):
     assert qvp.last_error()
 
 
+@pytest.mark.parametrize("call,arrays", [(_append, ["query_lens", "inv_freq", "rope_positions"]),
+                                         (_summarize, ["first_tokens"]), (_select, ["selected"]),
+                                         (_attend, ["selected"])])
+def test_misaligned_arrays_are_refused(call, arrays):
+    for name in arrays + ["block_tables", "context_lens", "error_word"]:
+        for off in (1, 2):
+            assert call(**{name: 0xe000 + off}) == qvp.ERR_INVALID, name
+            assert "aligned" in qvp.last_error()
+
+
 @pytest.mark.parametrize("call", [_append, _summarize, _select, _attend])
 def test_what_the_kernels_do_not_cover_is_refused(call):
     wide = qvp.make_shape(16, 2, 2, 264, 2)
