@@ -2,8 +2,8 @@
 // of the block score. Bound by HBM: K is read once (a summary is 2 /
 // tokens_per_block of it), so a thread owns one 16-byte column of a block's
 // token rows and has the loads of four slots in flight. Measured: 64 contexts
-// of 512 to 8,192 tokens (4 heads of 128, 312 MB in bf16) 51.9 us, 6.0 TB/s, in
-// fp32 101 us, 6.7 TB/s; 4 short fp32 ones 2.7 us. Eight slots and 256 threads:
+// of 512 to 8,192 tokens (4 heads of 128, 312 MB in bf16) 51.9 us, 6.0 TB/s, others
+// of the same range in fp32 (678 MB) 101 us, 6.7 TB/s; 4 short fp32 ones 2.7 us. Eight slots and 256 threads:
 // 52.6, 107.6 and 3.4.
 #include "sparse_common.cuh"
 
